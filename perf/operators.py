@@ -382,8 +382,9 @@ def _own(s):
         y = kernels.ssm(*operands, **more)
     else:
         act = None if s["form"] == "none" else "silu"
-        y = kernels.group_norm(s["x"], s["groups"], s["weight"], s["bias"], gate=s["gate"],
-                               activation=act, eps=EPS)
+        # heads apart: the last two dimensions are the groups
+        y = kernels.group_norm(s["x"], None if s["heads"] else s["groups"], s["weight"],
+                               s["bias"], gate=s["gate"], activation=act, eps=EPS)
     if form != "train":
         return y
     return [y, *torch.autograd.grad(y, [s[name] for name in s["leaves"]], s["dy"])]
