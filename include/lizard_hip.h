@@ -32,7 +32,7 @@
 extern "C" {
 #endif
 
-#define LZ_ABI_VERSION 16
+#define LZ_ABI_VERSION 17
 
 /*
  * gate_mode of the GLA entry points: a combination of
@@ -388,6 +388,123 @@ int lz_layer_combine_bwd(const void* dout, const void* y_swa, const float* alpha
                          void* dy_swa, float* dalpha, int out_bf16, int batch, int heads,
                          int length, int head_dim, void* workspace, size_t workspace_bytes,
                          void* stream);
+
+/*
+ * ---------------------------------------------------------------------------
+ * Recurrent mixers with a decay per channel and state, and what stands around
+ * them: the short causal convolution, the selective state space scan and the
+ * group norm.  No counterpart in the reference, whose recurrent mixer is gla.
+ *
+ * Activations are bf16 or fp32 (`bf16` != 0 or 0), all of a call in the one
+ * type; parameters, their gradients and recurrent states are fp32.  Inputs
+ * [batch, length, channels] may be slices of wider rows: channels lie next to
+ * each other, sequences and tokens `*_batch` and `*_token` elements apart
+ * (token and group strides at most LZ_MIXER_MAX_STRIDE).  Outputs are
+ * contiguous.  `lengths` (int [batch], or NULL) are the lengths of a padded
+ * batch's sequences, taken into [0, length]: outputs past them are zeros and
+ * the states are those after them.
+ * ---------------------------------------------------------------------------
+ */
+#define LZ_MIXER_MAX_STRIDE (1 << 24)
+#define LZ_SSM_MAX_STATE 64
+#define LZ_CONV_MAX_TAPS 4
+#define LZ_NORM_MAX_WIDTH 8192
+
+/*
+ * Operands of the selective state space scan, for each channel e of group
+ * e / (channels / groups):
+ *   delta_t = softplus(dt_t + dt_bias) (or without softplus),
+ *   h_t[n]  = exp(delta_t A[e, n]) h_{t-1}[n] + delta_t x_t B_t[n],
+ *   y_t     = (sum_n C_t[n] h_t[n] + D x_t) silu(z_t)
+ * A [channels, state]; D, dt_bias [channels] and z may be NULL.  B and C are
+ * [batch, length, groups, state], the state's entries next to each other.
+ */
+typedef struct {
+  const void *x, *dt, *z, *B, *C;
+  const float *A, *D, *dt_bias;
+  long long x_batch, dt_batch, z_batch, B_batch, C_batch;
+  long long x_token, dt_token, z_token, B_token, C_token;
+  long long B_group, C_group;
+  int batch, length, channels, state, groups;
+  int softplus, bf16;
+} lz_ssm_args;
+
+/* Bytes of the states lz_ssm_fwd keeps for lz_ssm_bwd (one every 16 tokens). */
+size_t lz_ssm_states_bytes(int batch, int length, int channels, int state);
+/* Workspace bytes of lz_ssm_fwd: the segments' own states, 0 when the
+ * sequences' channels alone fill the GPU. */
+size_t lz_ssm_fwd_workspace_bytes(int batch, int length, int channels, int state, int groups);
+/*
+ * The scan over whole sequences.  state_in (NULL: zeros) and state_out (NULL:
+ * not kept) are f32 [batch, channels, state], the states before the first and
+ * after the last token; they may not overlap.  states, of
+ * lz_ssm_states_bytes(), is written for lz_ssm_bwd, or NULL.
+ */
+int lz_ssm_fwd(const lz_ssm_args* args, const float* state_in, float* state_out,
+               const int* lengths, void* y, float* states, void* workspace,
+               size_t workspace_bytes, void* stream);
+/* One token of each sequence (length and the token strides are not read),
+ * the state updated in place. */
+int lz_ssm_decode_step(const lz_ssm_args* args, float* state, void* y, void* stream);
+/* Workspace bytes of lz_ssm_bwd. */
+size_t lz_ssm_bwd_workspace_bytes(int batch, int length, int channels, int state, int groups);
+/*
+ * Gradients of lz_ssm_fwd without state_in and lengths, from its states.
+ * dx, ddt, dz (with z), dB, dC in the activations' type; dA, dD (NULL without
+ * D), ddt_bias (likewise) f32.  No atomics: the same bits every time.
+ */
+int lz_ssm_bwd(const lz_ssm_args* args, const float* states, const void* dy, void* dx, void* ddt,
+               void* dz, void* dB, void* dC, float* dA, float* dD, float* ddt_bias,
+               void* workspace, size_t workspace_bytes, void* stream);
+
+/*
+ * Short causal convolution over the tokens of each channel,
+ *   y_t = act(bias + sum_j weight[c, j] x_{t - taps + 1 + j}),
+ * act silu or none; weight f32 [channels, taps], bias f32 or NULL.  state_in
+ * (NULL: zeros) and state_out (NULL: not kept) are the taps - 1 rows before
+ * the first and up to the last token, [batch, taps - 1, channels] in x's type;
+ * they may not overlap.
+ */
+int lz_short_conv_fwd(const void* x, long long x_batch, long long x_token, const float* weight,
+                      const float* bias, const void* state_in, void* state_out,
+                      const int* lengths, void* y, int batch, int length, int channels, int taps,
+                      int silu, int bf16, void* stream);
+/* One token of each sequence, the kept rows moved up in place. */
+int lz_short_conv_decode_step(const void* x, long long x_batch, const float* weight,
+                              const float* bias, void* state, void* y, int batch, int channels,
+                              int taps, int silu, int bf16, void* stream);
+size_t lz_short_conv_bwd_workspace_bytes(int batch, int length, int channels, int taps);
+/* Gradients of lz_short_conv_fwd without states and lengths; dbias NULL
+ * without bias. */
+int lz_short_conv_bwd(const void* x, long long x_batch, long long x_token, const float* weight,
+                      const float* bias, const void* dy, void* dx, float* dweight, float* dbias,
+                      int batch, int length, int channels, int taps, int silu, int bf16,
+                      void* workspace, size_t workspace_bytes, void* stream);
+
+/*
+ * Operands of the group norm of each token's `groups` groups of `width`
+ * channels: n = (x - mean) / sqrt(var + eps) over a group, o = n weight + bias,
+ * y = o, silu(o), o gate or o silu(gate) (`silu`, gate).  weight and bias f32
+ * [groups * width], each may be NULL; x and gate [batch, length, groups,
+ * width] with their strides, a group's channels next to each other.
+ */
+typedef struct {
+  const void *x, *gate;
+  const float *weight, *bias;
+  long long x_batch, x_token, x_group, gate_batch, gate_token, gate_group;
+  int batch, length, groups, width;
+  int silu, bf16;
+  float eps;
+} lz_group_norm_args;
+
+/* y [batch, length, groups, width]. */
+int lz_group_norm_fwd(const lz_group_norm_args* args, void* y, void* stream);
+size_t lz_group_norm_bwd_workspace_bytes(int batch, int length, int groups, int width);
+/* Gradients: dx, dgate (with gate) in the activations' type, dweight and dbias
+ * f32 (NULL: not formed). */
+int lz_group_norm_bwd(const lz_group_norm_args* args, const void* dy, void* dx, void* dgate,
+                      float* dweight, float* dbias, void* workspace, size_t workspace_bytes,
+                      void* stream);
 
 #ifdef __cplusplus
 }

@@ -8,12 +8,13 @@ import os
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(_HERE, "_lib", "liblizard_hip.so")
-ABI_VERSION = 16
+ABI_VERSION = 17
 
 _P = ctypes.c_void_p
 _I = ctypes.c_int
 _F = ctypes.c_float
 _S = ctypes.c_size_t
+_L = ctypes.c_longlong
 
 # name -> (restype, argtypes); must match include/lizard_hip.h
 SIGNATURES = {
@@ -47,7 +48,38 @@ SIGNATURES = {
     "lz_layer_combine_fwd": (_I, [_P, _P, _P, _P, _I, _I, _I, _I, _I, _P]),
     "lz_layer_combine_bwd_workspace_bytes": (_S, []),
     "lz_layer_combine_bwd": (_I, [_P, _P, _P, _P, _P, _P, _I, _I, _I, _I, _I, _P, _S, _P]),
+    "lz_ssm_states_bytes": (_S, [_I, _I, _I, _I]),
+    "lz_ssm_fwd_workspace_bytes": (_S, [_I, _I, _I, _I, _I]),
+    "lz_ssm_fwd": (_I, [_P, _P, _P, _P, _P, _P, _P, _S, _P]),
+    "lz_ssm_decode_step": (_I, [_P, _P, _P, _P]),
+    "lz_ssm_bwd_workspace_bytes": (_S, [_I, _I, _I, _I, _I]),
+    "lz_ssm_bwd": (_I, [_P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _S, _P]),
+    "lz_short_conv_fwd": (_I, [_P, _L, _L, _P, _P, _P, _P, _P, _P, _I, _I, _I, _I, _I, _I, _P]),
+    "lz_short_conv_decode_step": (_I, [_P, _L, _P, _P, _P, _P, _I, _I, _I, _I, _I, _P]),
+    "lz_short_conv_bwd_workspace_bytes": (_S, [_I, _I, _I, _I]),
+    "lz_short_conv_bwd": (_I, [_P, _L, _L, _P, _P, _P, _P, _P, _P, _I, _I, _I, _I, _I, _I, _P,
+                               _S, _P]),
+    "lz_group_norm_fwd": (_I, [_P, _P, _P]),
+    "lz_group_norm_bwd_workspace_bytes": (_S, [_I, _I, _I, _I]),
+    "lz_group_norm_bwd": (_I, [_P, _P, _P, _P, _P, _P, _P, _S, _P]),
 }
+
+
+class SsmArgs(ctypes.Structure):
+    """lz_ssm_args"""
+    _fields_ = [(n, _P) for n in ("x", "dt", "z", "B", "C", "A", "D", "dt_bias")] + \
+        [(f"{n}_batch", _L) for n in ("x", "dt", "z", "B", "C")] + \
+        [(f"{n}_token", _L) for n in ("x", "dt", "z", "B", "C")] + \
+        [("B_group", _L), ("C_group", _L)] + \
+        [(n, _I) for n in ("batch", "length", "channels", "state", "groups", "softplus", "bf16")]
+
+
+class GroupNormArgs(ctypes.Structure):
+    """lz_group_norm_args"""
+    _fields_ = [(n, _P) for n in ("x", "gate", "weight", "bias")] + \
+        [(f"{n}_{d}", _L) for n in ("x", "gate") for d in ("batch", "token", "group")] + \
+        [(n, _I) for n in ("batch", "length", "groups", "width", "silu", "bf16")] + [("eps", _F)]
+
 
 _lib = None
 

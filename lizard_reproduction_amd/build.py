@@ -4,9 +4,9 @@ it with g++ (in-tree, no JIT cache).
     python -m lizard_reproduction_amd.build
 
 Each .hip source in csrc/ is compiled to an object in parallel, then linked
-into ``lizard_reproduction_amd/_lib/liblizard_hip.so``; csrc/torch_ops.cpp, host
-code against torch's headers, becomes ``_lib/lizard_torch.so``, which finds the
-library beside itself.
+into ``lizard_reproduction_amd/_lib/liblizard_hip.so``; csrc/torch_ops.cpp and
+csrc/mixer_ops.cpp, host code against torch's headers, become
+``_lib/lizard_torch.so``, which finds the library beside itself.
 """
 import concurrent.futures
 import os
@@ -20,6 +20,7 @@ CSRC = os.path.join(HERE, "csrc")
 LIBDIR = os.path.join(HERE, "_lib")
 LIBNAME = "liblizard_hip.so"
 MODULENAME = "lizard_torch.so"
+MODULE_SOURCES = ("torch_ops", "mixer_ops")
 ARCH = "gfx950"
 
 HIPCC_FLAGS = [
@@ -64,11 +65,11 @@ def _compile_module(src, obj):
     return obj
 
 
-def _link_module(obj):
+def _link_module(objs):
     from torch.utils import cpp_extension
     out = os.path.join(LIBDIR, MODULENAME)
     tmp = out + ".tmp"
-    cmd = ["g++", "-shared", "-fPIC", obj, "-o", tmp,
+    cmd = ["g++", "-shared", "-fPIC", *objs, "-o", tmp,
            *(f"-L{path}" for path in cpp_extension.library_paths("cuda")), "-L" + LIBDIR,
            "-l:" + LIBNAME, "-lc10", "-lc10_hip", "-ltorch_cpu", "-ltorch_hip", "-ltorch",
            "-ltorch_python", "-Wl,-rpath,$ORIGIN"]
@@ -87,12 +88,14 @@ def build(verbose=True):
     os.makedirs(LIBDIR, exist_ok=True)
     srcs = sources()
     objs = [os.path.join(objdir, os.path.basename(s)[:-4] + ".o") for s in srcs]
-    module_obj = os.path.join(objdir, "torch_ops.o")
-    workers = min(len(srcs) + 1, max(1, (os.cpu_count() or 4)))
+    module_objs = [os.path.join(objdir, name + ".o") for name in MODULE_SOURCES]
+    workers = min(len(srcs) + len(module_objs), max(1, (os.cpu_count() or 4)))
     with concurrent.futures.ThreadPoolExecutor(workers) as pool:
-        module = pool.submit(_compile_module, os.path.join(CSRC, "torch_ops.cpp"), module_obj)
+        module = [pool.submit(_compile_module, os.path.join(CSRC, name + ".cpp"), obj)
+                  for name, obj in zip(MODULE_SOURCES, module_objs)]
         list(pool.map(_compile, srcs, objs))
-        module.result()
+        for job in module:
+            job.result()
     out = os.path.join(LIBDIR, LIBNAME)
     tmp = out + ".tmp"
     cmd = [hipcc(), f"--offload-arch={ARCH}", "-shared", "-fPIC", *objs, "-o", tmp]
@@ -100,7 +103,7 @@ def build(verbose=True):
     if proc.returncode != 0:
         raise RuntimeError(f"link failed:\n{proc.stderr}")
     os.replace(tmp, out)
-    module_out = _link_module(module_obj)
+    module_out = _link_module(module_objs)
     if verbose:
         print(f"built {out} and {module_out}")
     return out

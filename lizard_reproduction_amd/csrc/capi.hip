@@ -7,6 +7,7 @@
 #include <string>
 
 #include "../../include/lizard_hip.h"
+#include "capi.hpp"
 #include "common.hpp"
 
 namespace lz {
@@ -83,8 +84,7 @@ hipError_t launch_combine_bwd(const void* dout, const void* ys, const float* alp
 
 static thread_local std::string g_err;
 
-static int fail(int code, const char* fmt, ...) __attribute__((format(printf, 2, 3)));
-static int fail(int code, const char* fmt, ...) {
+int lz::fail(int code, const char* fmt, ...) {
   char buf[512];
   va_list ap;
   va_start(ap, fmt);
@@ -94,13 +94,16 @@ static int fail(int code, const char* fmt, ...) {
   return code;
 }
 
-static int hip_status(hipError_t e, const char* what) {
+int lz::hip_status(hipError_t e, const char* what) {
   if (e == hipSuccess) {
     g_err.clear();
     return 0;
   }
   return fail((int)e, "%s: HIP error %d (%s)", what, (int)e, hipGetErrorString(e));
 }
+
+using lz::fail;
+using lz::hip_status;
 
 static bool pow2_at_least_16(int c) { return c >= 16 && (c & (c - 1)) == 0; }
 

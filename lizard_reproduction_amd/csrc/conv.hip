@@ -1,0 +1,277 @@
+// Short causal convolution over the tokens of each channel, channels last:
+//
+//   pre_t = bias + sum_{j < K} w_j x_{t-K+1+j},   y_t = pre_t or silu(pre_t)
+//
+// K is at most four, so a value takes a few operations and the bytes of x and y (backward:
+// x, dy, y's recomputation and dx) bound it.  A thread takes eight channels and a run of
+// tokens, with the K rows in registers: a row is read once by the run it lies in and again,
+// from cache, by the run after it.  A workgroup's threads are columns of eight channels
+// times runs, a row's columns next to each other.
+//
+// Backward: g_t = dy_t act'(pre_t), dx_t = sum_j w_j g_{t+K-1-j} (the run goes K - 1 tokens
+// on), dw_j = sum_t g_t x_{t-K+1+j}, dbias = sum_t g_t: the workgroup's runs meet in LDS and
+// its shares go to a second launch, which adds them in order.
+#include "conv.hpp"
+
+namespace lz {
+
+// Where a thread works: its columns, and its run of tokens of a sequence
+struct ConvPlace {
+  int col, run, b, t0, left;
+  bool in;
+  __device__ __forceinline__ ConvPlace(const Conv& p) {
+    col = (blockIdx.y * p.cols + threadIdx.x % p.cols) * 8;
+    run = blockIdx.x * (CONV_THREADS / p.cols) + threadIdx.x / p.cols;
+    in = col < p.C && run < p.batch * p.seq_runs;
+    if (!in) col = 0, run = 0;
+    b = run / p.seq_runs;
+    t0 = (run - b * p.seq_runs) * p.run;
+    left = p.C - col;
+  }
+};
+
+template <int K>
+__device__ __forceinline__ void load_taps(const Conv& p, int col, int left, float (&w)[K][8],
+                                          float (&bias)[8]) {
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const int c = col + (i < left ? i : 0);
+#pragma unroll
+    for (int j = 0; j < K; ++j) w[j][i] = p.w[(size_t)c * K + j];
+    bias[i] = p.bias ? p.bias[c] : 0.f;
+  }
+}
+
+// Row t of sequence b, from the kept state where t < 0 (zeros without one)
+template <typename T, bool VEC, int K>
+__device__ __forceinline__ void row_before(const Conv& p, const T* xb, int b, int t, int col,
+                                           int left, float (&v)[8]) {
+  Cols8<T, VEC> c;
+  const T* state = (const T*)p.state_in;
+  const bool have = t >= 0 || state;
+  const T* from = t >= 0 || !state ? xb + (long long)max(t, 0) * p.x_t
+                                   : state + ((long long)b * (K - 1) + (t + K - 1)) * p.C + col;
+  c.load(from, left);
+#pragma unroll
+  for (int i = 0; i < 8; ++i) v[i] = have ? c.r.at(i) : 0.f;
+}
+
+constexpr int CONV_AHEAD = 4;   // rows loaded before the first of them is used
+
+template <typename T, bool VEC, int K>
+__global__ __launch_bounds__(CONV_THREADS) void conv_fwd_kernel(Conv p) {
+  const ConvPlace at(p);
+  if (!at.in) return;
+  const int len = p.lengths ? max(0, min(p.L, p.lengths[at.b])) : p.L;
+  const T* xb = (const T*)p.x + at.b * p.x_b + at.col;
+  T* yb = (T*)p.y + (long long)at.b * p.L * p.C + at.col;
+  float w[K][8], bias[8], win[K][8];   // win[j]: row t - K + 1 + j
+  load_taps<K>(p, at.col, at.left, w, bias);
+#pragma unroll
+  for (int j = 1; j < K; ++j)
+    row_before<T, VEC, K>(p, xb, at.b, at.t0 + j - K, at.col, at.left, win[j]);
+  const int t1 = min(at.t0 + p.run, p.L);
+  for (int t = at.t0; t < t1; t += CONV_AHEAD) {
+    Cols8<T, VEC> next[CONV_AHEAD];
+#pragma unroll
+    for (int i = 0; i < CONV_AHEAD; ++i)
+      next[i].load(xb + (long long)min(t + i, p.L - 1) * p.x_t, at.left);
+#pragma unroll
+    for (int i = 0; i < CONV_AHEAD; ++i) {
+      Cols8<T, VEC> out;
+#pragma unroll
+      for (int c = 0; c < 8; ++c) {
+#pragma unroll
+        for (int j = 0; j + 1 < K; ++j) win[j][c] = win[j + 1][c];
+        win[K - 1][c] = next[i].r.at(c);
+        float y = bias[c];
+#pragma unroll
+        for (int j = 0; j < K; ++j) y = fmaf(w[j][c], win[j][c], y);
+        if (p.act) y *= sigmoid(y);
+        out.r.set(c, t + i < len ? y : 0.f);
+      }
+      if (t + i < t1) out.store(yb + (long long)(t + i) * p.C, at.left);
+    }
+  }
+  // the last K - 1 rows of the sequence, by the run that begins it
+  if (K > 1 && p.state_out && at.t0 == 0) {
+#pragma unroll
+    for (int j = 0; j < K - 1; ++j) {
+      float v[8];
+      row_before<T, VEC, K>(p, xb, at.b, len - (K - 1) + j, at.col, at.left, v);
+      Cols8<T, VEC> out;
+#pragma unroll
+      for (int c = 0; c < 8; ++c) out.r.set(c, v[c]);
+      out.store((T*)p.state_out + ((long long)at.b * (K - 1) + j) * p.C + at.col, at.left);
+    }
+  }
+}
+
+// One token of each sequence: a thread a channel, its kept rows moved up in place
+template <typename T, int K>
+__global__ __launch_bounds__(256) void conv_step_kernel(Conv p) {
+  const int c = blockIdx.x * 256 + threadIdx.x, b = blockIdx.y;
+  if (c >= p.C) return;
+  T* state = (T*)p.state_out + (long long)b * (K - 1) * p.C + c;
+  T row[K];
+#pragma unroll
+  for (int j = 0; j < K - 1; ++j) row[j] = state[(long long)j * p.C];
+  row[K - 1] = ((const T*)p.x)[b * p.x_b + c];
+  float y = p.bias ? p.bias[c] : 0.f;
+#pragma unroll
+  for (int j = 0; j < K; ++j) y = fmaf(p.w[(size_t)c * K + j], (float)row[j], y);
+#pragma unroll
+  for (int j = 0; j < K - 1; ++j) state[(long long)j * p.C] = row[j + 1];
+  if (p.act) y *= sigmoid(y);
+  ((T*)p.y)[(long long)b * p.C + c] = (T)y;
+}
+
+template <typename T, bool VEC, int K>
+__global__ __launch_bounds__(CONV_THREADS) void conv_bwd_kernel(Conv p, const void* dy_, void* dx_,
+                                                                float* part) {
+  __shared__ float red[CONV_THREADS][9];
+  const ConvPlace at(p);
+  const T* xb = (const T*)p.x + at.b * p.x_b + at.col;
+  const T* dyb = (const T*)dy_ + (long long)at.b * p.L * p.C + at.col;
+  T* dxb = (T*)dx_ + (long long)at.b * p.L * p.C + at.col;
+  float w[K][8], bias[8], win[K][8], g[K][8];   // g[j]: the gradient at token t - K + 1 + j
+  float dw[K][8], dbias[8];
+  load_taps<K>(p, at.col, at.left, w, bias);
+#pragma unroll
+  for (int c = 0; c < 8; ++c) {
+    dbias[c] = 0.f;
+#pragma unroll
+    for (int j = 0; j < K; ++j) dw[j][c] = g[j][c] = 0.f;
+  }
+#pragma unroll
+  for (int j = 1; j < K; ++j)
+    row_before<T, VEC, K>(p, xb, at.b, at.t0 + j - K, at.col, at.left, win[j]);
+  const int t1 = at.in ? min(at.t0 + p.run, p.L) : at.t0;   // the run's tokens,
+  const int t2 = at.in ? t1 + K - 1 : at.t0;                // and those their dx comes from
+  for (int t = at.t0; t < t2; t += CONV_AHEAD) {
+    Cols8<T, VEC> next[CONV_AHEAD], dy[CONV_AHEAD];
+#pragma unroll
+    for (int i = 0; i < CONV_AHEAD; ++i) {
+      const long long row = min(t + i, p.L - 1);
+      next[i].load(xb + row * p.x_t, at.left);
+      dy[i].load(dyb + row * p.C, at.left);
+    }
+#pragma unroll
+    for (int i = 0; i < CONV_AHEAD; ++i) {
+      Cols8<T, VEC> out;
+      const bool own = t + i < t1, there = t + i < p.L;
+#pragma unroll
+      for (int c = 0; c < 8; ++c) {
+#pragma unroll
+        for (int j = 0; j + 1 < K; ++j) win[j][c] = win[j + 1][c], g[j][c] = g[j + 1][c];
+        win[K - 1][c] = next[i].r.at(c);
+        float d = dy[i].r.at(c);
+        if (p.act) {
+          float pre = bias[c];
+#pragma unroll
+          for (int j = 0; j < K; ++j) pre = fmaf(w[j][c], win[j][c], pre);
+          const float s = sigmoid(pre);
+          d *= s * fmaf(pre, 1.f - s, 1.f);
+        }
+        d = there ? d : 0.f;
+        g[K - 1][c] = d;
+        const float mine = own ? d : 0.f;
+        dbias[c] += mine;
+        float dx = 0.f;
+#pragma unroll
+        for (int j = 0; j < K; ++j) {
+          dw[j][c] = fmaf(mine, own ? win[j][c] : 0.f, dw[j][c]);
+          dx = fmaf(w[j][c], g[K - 1 - j][c], dx);   // g at token t - j: tap K - 1 - j
+        }
+        out.r.set(c, dx);
+      }
+      (void)out;
+      if (t + i - (K - 1) >= at.t0 && t + i - (K - 1) < t1)
+        out.store(dxb + (long long)(t + i - (K - 1)) * p.C, at.left);
+    }
+  }
+  // the workgroup's runs, one sum at a time: [K + 1][C] floats a row of workgroups
+  const int runs = CONV_THREADS / p.cols;
+#pragma unroll
+  for (int j = 0; j <= K; ++j) {
+    __syncthreads();
+#pragma unroll
+    for (int c = 0; c < 8; ++c) red[threadIdx.x][c] = j < K ? dw[j < K ? j : 0][c] : dbias[c];
+    __syncthreads();
+    for (int i = threadIdx.x; i < 8 * p.cols; i += CONV_THREADS) {
+      const int ch = blockIdx.y * p.cols * 8 + i;
+      if (ch >= p.C) continue;
+      float sum = 0.f;
+      for (int r = 0; r < runs; ++r) sum += red[r * p.cols + i / 8][i % 8];
+      part[((size_t)blockIdx.x * (K + 1) + j) * p.C + ch] = sum;
+    }
+  }
+}
+
+// Runs long enough that their K - 1 rows before them cost little, short enough that the
+// threads fill the chip twice over
+void conv_split(Conv& p) {
+  const int vecs = (p.C + 7) / 8;
+  int cols = 1;
+  while (cols < 64 && cols < vecs) cols *= 2;
+  p.cols = cols;
+  p.col_blocks = (vecs + cols - 1) / cols;
+  const long long rows = (long long)p.batch * p.L;
+  const long long threads = 512LL * device_geom().cus;
+  long long run = rows * vecs / threads;
+  run = run < 8 ? 8 : run > 64 ? 64 : run;
+  run = (run + CONV_AHEAD - 1) / CONV_AHEAD * CONV_AHEAD;
+  p.run = (int)run;
+  p.seq_runs = (int)((p.L + run - 1) / run);
+  const long long all = (long long)p.batch * p.seq_runs, per = CONV_THREADS / cols;
+  p.run_blocks = (int)((all + per - 1) / per);
+}
+
+template <typename T, bool VEC>
+hipError_t conv_taps(const Conv& p, int K, const void* dy, void* dx, float* part, hipStream_t st) {
+  const dim3 grid(p.run_blocks, p.col_blocks), block(CONV_THREADS);
+#define LZ_TAPS(k)                                                                        \
+  if (K == k) {                                                                           \
+    if (dy) hipLaunchKernelGGL((conv_bwd_kernel<T, VEC, k>), grid, block, 0, st, p, dy, dx, part); \
+    else hipLaunchKernelGGL((conv_fwd_kernel<T, VEC, k>), grid, block, 0, st, p);         \
+  }
+  LZ_TAPS(1) LZ_TAPS(2) LZ_TAPS(3) LZ_TAPS(4)
+#undef LZ_TAPS
+  return hipGetLastError();
+}
+
+hipError_t launch_conv(const Conv& p, int K, const void* dy, void* dx, float* part, bool is_bf16,
+                       bool vec, hipStream_t st) {
+  if (is_bf16)
+    return vec ? conv_taps<bf16, true>(p, K, dy, dx, part, st)
+               : conv_taps<bf16, false>(p, K, dy, dx, part, st);
+  return vec ? conv_taps<float, true>(p, K, dy, dx, part, st)
+             : conv_taps<float, false>(p, K, dy, dx, part, st);
+}
+
+hipError_t launch_conv_sums(const Conv& p, int K, const float* part, float* dw, float* dbias,
+                            hipStream_t st) {
+  SumJobs jobs = {};
+  // part [parts][K + 1][C] -> dw [C, K], dbias [C]
+  jobs.job[jobs.n++] = SumJob{part, dw, (long long)(K + 1) * p.C, p.C, 1, K, K, p.C, p.run_blocks, 0};
+  if (dbias)
+    jobs.job[jobs.n++] = SumJob{part + (size_t)K * p.C, dbias, (long long)(K + 1) * p.C, 0, 0, 1, 1,
+                                p.C, p.run_blocks, 0};
+  return launch_sums(jobs, st);
+}
+
+template <typename T>
+hipError_t step_taps(const Conv& p, int K, hipStream_t st) {
+  const dim3 grid((p.C + 255) / 256, p.batch);
+#define LZ_TAPS(k) \
+  if (K == k) hipLaunchKernelGGL((conv_step_kernel<T, k>), grid, dim3(256), 0, st, p);
+  LZ_TAPS(1) LZ_TAPS(2) LZ_TAPS(3) LZ_TAPS(4)
+#undef LZ_TAPS
+  return hipGetLastError();
+}
+
+hipError_t launch_conv_step(const Conv& p, int K, bool is_bf16, hipStream_t st) {
+  return is_bf16 ? step_taps<bf16>(p, K, st) : step_taps<float>(p, K, st);
+}
+
+}  // namespace lz

@@ -1,0 +1,30 @@
+// Arguments of the short convolution's kernels (conv.hip).
+#pragma once
+#include "mixer_common.hpp"
+
+namespace lz {
+
+constexpr int CONV_THREADS = 256, CONV_MAX_TAPS = 4;
+
+struct Conv {
+  const void* x;
+  const float *w, *bias;         // [C, K], [C]
+  const void* state_in;          // [B, K - 1, C], the rows before the first
+  void* state_out;
+  const int* lengths;
+  void* y;                       // [B, L, C]
+  long long x_b;                 // elements from one sequence to the next
+  int x_t;                       // and from one token to the next
+  int batch, L, C, act;
+  // conv_split: columns (of eight channels) a workgroup, tokens a run, runs a sequence
+  int cols, col_blocks, run, seq_runs, run_blocks;
+};
+
+void conv_split(Conv& p);
+hipError_t launch_conv(const Conv& p, int K, const void* dy, void* dx, float* part, bool is_bf16,
+                       bool vec, hipStream_t st);
+hipError_t launch_conv_sums(const Conv& p, int K, const float* part, float* dw, float* dbias,
+                            hipStream_t st);
+hipError_t launch_conv_step(const Conv& p, int K, bool is_bf16, hipStream_t st);
+
+}  // namespace lz

@@ -1,0 +1,197 @@
+// What the recurrent mixers' operators share (ssm.hip, conv.hip, norm.hip): rows of
+// bf16 or fp32 elements read and written through buffer resources, activations in
+// fp32, and the sum of partial results in a fixed order.
+#pragma once
+#include "common.hpp"
+
+namespace lz {
+
+template <typename T>
+constexpr bool IS_BF16 = sizeof(T) == 2;
+
+// V consecutive elements of a row as loaded: packed words where the loads are vectors
+// (VEC), else a word an element.  They stay packed until they are used, so that a load
+// made a tile ahead holds few registers and nothing waits for it.
+template <typename T, int V, bool VEC>
+struct RawRow {
+  static constexpr int WORDS = VEC ? (V * (int)sizeof(T) + 3) / 4 : V;
+  uint32_t w[WORDS];
+
+  __device__ __forceinline__ float at(int i) const {
+    if constexpr (!IS_BF16<T>) return __builtin_bit_cast(float, w[i]);
+    else if constexpr (!VEC) return __builtin_bit_cast(float, w[i] << 16);
+    else return __builtin_bit_cast(float, (i & 1) ? w[i >> 1] & 0xffff0000u : w[i >> 1] << 16);
+  }
+  __device__ __forceinline__ void set(int i, float x) {
+    if constexpr (!IS_BF16<T>) {
+      w[i] = __builtin_bit_cast(uint32_t, x);
+    } else {
+      const uint32_t h = __builtin_bit_cast(uint16_t, to_bf16(x));
+      if constexpr (!VEC) w[i] = h;
+      else if (i & 1) w[i >> 1] |= h << 16;
+      else w[i >> 1] = h;
+    }
+  }
+};
+
+// Elements [off, off + V) (in elements from the resource's base), zeros where !in or
+// from element `left` of them on (what lies past a row's channels).
+template <typename T, int V, bool VEC>
+__device__ __forceinline__ RawRow<T, V, VEC> load_raw(rsrc_t r, uint32_t off, bool in, int left) {
+  RawRow<T, V, VEC> o;
+  constexpr int S = sizeof(T);
+  if constexpr (VEC) {
+    const uint32_t at = in && left > 0 ? off * S : OOB;
+    constexpr int B = V * S;
+    if constexpr (B == 2) {
+      o.w[0] = __builtin_amdgcn_raw_buffer_load_b16(r, at, 0, 0);
+    } else if constexpr (B == 4) {
+      o.w[0] = __builtin_amdgcn_raw_buffer_load_b32(r, at, 0, 0);
+    } else if constexpr (B == 8) {
+      const auto v = __builtin_bit_cast(uint2, __builtin_amdgcn_raw_buffer_load_b64(r, at, 0, 0));
+      o.w[0] = v.x, o.w[1] = v.y;
+    } else {
+#pragma unroll
+      for (int k = 0; k < B / 16; ++k) {
+        const uint4 v = bload16(r, at + 16 * k);
+        o.w[4 * k] = v.x, o.w[4 * k + 1] = v.y, o.w[4 * k + 2] = v.z, o.w[4 * k + 3] = v.w;
+      }
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+      const uint32_t at = in && i < left ? (off + i) * S : OOB;
+      if constexpr (S == 2) o.w[i] = __builtin_amdgcn_raw_buffer_load_b16(r, at, 0, 0);
+      else o.w[i] = __builtin_amdgcn_raw_buffer_load_b32(r, at, 0, 0);
+    }
+  }
+  return o;
+}
+
+template <typename T, int V, bool VEC>
+__device__ __forceinline__ void store_raw(rsrc_t r, uint32_t off, bool in, int left,
+                                          const RawRow<T, V, VEC>& o) {
+  constexpr int S = sizeof(T);
+  if constexpr (VEC) {
+    const uint32_t at = in && left > 0 ? off * S : OOB;
+    constexpr int B = V * S;
+    if constexpr (B == 2) {
+      __builtin_amdgcn_raw_buffer_store_b16((uint16_t)o.w[0], r, at, 0, 0);
+    } else if constexpr (B == 4) {
+      __builtin_amdgcn_raw_buffer_store_b32(o.w[0], r, at, 0, 0);
+    } else if constexpr (B == 8) {
+      typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+      __builtin_amdgcn_raw_buffer_store_b64(u32x2{o.w[0], o.w[1]}, r, at, 0, 0);
+    } else {
+#pragma unroll
+      for (int k = 0; k < B / 16; ++k)
+        __builtin_amdgcn_raw_buffer_store_b128(
+            u32x4{o.w[4 * k], o.w[4 * k + 1], o.w[4 * k + 2], o.w[4 * k + 3]}, r, at + 16 * k, 0, 0);
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+      const uint32_t at = in && i < left ? (off + i) * S : OOB;
+      if constexpr (S == 2) __builtin_amdgcn_raw_buffer_store_b16((uint16_t)o.w[i], r, at, 0, 0);
+      else __builtin_amdgcn_raw_buffer_store_b32(o.w[i], r, at, 0, 0);
+    }
+  }
+}
+
+// Eight channels of a row through a pointer of the lane's own.  Rows are clamped into the
+// tensor by the callers and what does not exist is selected away after the load, so no
+// branch holds loads apart.
+template <typename T, bool VEC>
+struct Cols8 {
+  RawRow<T, 8, VEC> r;
+  __device__ __forceinline__ void load(const T* p, int left) {
+    if constexpr (VEC) {
+#pragma unroll
+      for (int k = 0; k < (int)sizeof(T) / 2; ++k) {
+        const uint4 v = reinterpret_cast<const uint4*>(p)[k];
+        r.w[4 * k] = v.x, r.w[4 * k + 1] = v.y, r.w[4 * k + 2] = v.z, r.w[4 * k + 3] = v.w;
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const T v = p[i < left ? i : 0];
+        if constexpr (IS_BF16<T>) r.w[i] = __builtin_bit_cast(uint16_t, v);
+        else r.w[i] = __builtin_bit_cast(uint32_t, v);
+      }
+    }
+  }
+  __device__ __forceinline__ void store(T* p, int left) const {
+    if constexpr (VEC) {
+#pragma unroll
+      for (int k = 0; k < (int)sizeof(T) / 2; ++k)
+        reinterpret_cast<uint4*>(p)[k] =
+            uint4{r.w[4 * k], r.w[4 * k + 1], r.w[4 * k + 2], r.w[4 * k + 3]};
+    } else {
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+        if (i < left) p[i] = (T)r.at(i);
+    }
+  }
+};
+
+// A resource from base on that takes every offset under 2 GiB: the loads and stores here
+// pass OOB for what a row or a tile does not have.  Callers rebase it every few rows, in
+// 64 bits, so the 32-bit offsets within never pass a tile.
+template <typename T>
+__device__ __forceinline__ rsrc_t open_rsrc(const T* base) {
+  return __builtin_amdgcn_make_buffer_rsrc(const_cast<T*>(base), (short)0, 0x7fffffff, RSRC_WORD3);
+}
+
+__device__ __forceinline__ float sigmoid(float x) {
+  return __builtin_amdgcn_rcpf(1.f + fexp(-x));   // e^-x past fp32: 1 / inf = 0
+}
+
+// log(1 + e) for e in [0, 1]: 2 atanh(s) with s = e / (2 + e) <= 1/3, by its power series
+// up to s^15 (the next term is under 2^-29 of the sum).  The hardware's log of 1 + e
+// would lose e's low bits, and small steps are what a trained dt gives.
+__device__ __forceinline__ float log1p_unit(float e) {
+  const float s = e * __builtin_amdgcn_rcpf(2.f + e), q = s * s;
+  float p = 1.f / 15;
+  p = fmaf(p, q, 1.f / 13);
+  p = fmaf(p, q, 1.f / 11);
+  p = fmaf(p, q, 1.f / 9);
+  p = fmaf(p, q, 1.f / 7);
+  p = fmaf(p, q, 1.f / 5);
+  p = fmaf(p, q, 1.f / 3);
+  p = fmaf(p, q, 1.f);
+  return 2.f * s * p;
+}
+
+__device__ __forceinline__ float softplus(float x) {
+  return fmaxf(x, 0.f) + log1p_unit(fexp(-fabsf(x)));
+}
+
+// x of another lane of this lane's row of 16, or of its quad, as an operand of the
+// instruction that uses it (DPP).
+template <int CTRL>
+__device__ __forceinline__ float dpp(float x) {
+  return __builtin_bit_cast(
+      float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, x), CTRL, 0xf, 0xf, true));
+}
+constexpr int DPP_XOR1 = 0xb1, DPP_XOR2 = 0x4e;          // quad_perm [1,0,3,2], [2,3,0,1]
+constexpr int DPP_HALF_MIRROR = 0x141, DPP_ROR8 = 0x128; // lane 7 - i of its 8; lane i + 8 mod 16
+constexpr int DPP_BCAST = 0x150;                         // + k: lane k of the row, to all of it
+
+// Sums of partial results in the order of their index, by one launch.  A job sums, for
+// each of `rows` x `cols` outputs, `parts` values `part_stride` floats apart that begin
+// at src + row * row_stride + col; output (row, col) goes to
+// dst + row * out_row + col * out_col, as bf16 or float.
+struct SumJob {
+  const float* src;
+  void* dst;
+  long long part_stride, row_stride, out_row, out_col;
+  int rows, cols, parts, bf16;
+};
+constexpr int SUM_JOBS = 6;
+struct SumJobs {
+  SumJob job[SUM_JOBS];
+  int n;
+};
+hipError_t launch_sums(const SumJobs& jobs, hipStream_t st);
+
+}  // namespace lz

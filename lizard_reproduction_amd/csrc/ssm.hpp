@@ -1,0 +1,137 @@
+// Arguments of the selective state space scan's kernels (ssm.hip, ssm_bwd.hip) and the
+// walk over a tile that both directions begin with.
+#pragma once
+#include <utility>
+
+#include "mixer_common.hpp"
+
+namespace lz {
+
+// Layout of the work.  A workgroup takes 64 channels of one group and one sequence (or a
+// segment of it) and walks it in tiles of 16 tokens; a lane is a channel, and wave w of
+// its W holds the states n = 4 w .. 4 w + 3 (and 4 (w + W) .. with NP = 2), four a lane,
+// in registers.
+constexpr int SSM_CH = 64, SSM_TT = 16, SSM_MAX_STATE = 64;
+constexpr int SSM_PITCH = SSM_TT + 4;   // floats from one channel to the next in LDS: 16-byte
+                                        // reads of 16 lanes fall on all 64 banks
+constexpr int SSM_TILE = SSM_CH * SSM_PITCH;
+
+struct Ssm {
+  const void *x, *dt, *z, *B, *C;
+  const float *A, *D, *bias;
+  const float* state_in;
+  float* state_out;
+  const int* lengths;
+  void* y;
+  float* saved;    // [B, tiles, N, E]: the state before each tile, for the backward
+  float* rec;      // [B, S - 1, N, E]: a segment's own state, from zero
+  float* dsum;     // [B, S - 1, E]: its sum of delta
+  long long x_b, dt_b, z_b, B_b, C_b, y_b;   // elements from one sequence to the next
+  int x_t, dt_t, z_t, B_t, C_t;              // from one token to the next
+  int B_g, C_g;                              // from one group to the next
+  int batch, L, E, N, G, Eg, gblocks;        // gblocks: 64-channel blocks of a group
+  int tiles, seg_tiles, S, softplus;
+};
+
+// Gradients (ssm_bwd.hip)
+struct SsmGrad {
+  const void* dy;
+  void *dx, *ddt, *dz;   // [B, L, E]
+  float* part_bc;        // [blocks, B, L, 2, NQ]: a block's share of dB and dC
+  float* part_a;         // [B S, N, E]
+  float* part_d;         // [B S, 2, E]: of dD and ddt_bias
+  float* rec;            // as Ssm's, of the reverse walk
+  float* dsum;
+};
+
+// The V elements a thread takes of R rows of a tile, W waves to a workgroup
+template <int W>
+struct SsmSplit {
+  static constexpr int V = 16 / W < 8 ? 16 / W : 8;
+  static constexpr int R = 16 / (W * V);
+  static constexpr int COLS = SSM_CH / V;          // threads to a row
+  static constexpr int ROWS = 64 * W / COLS;       // rows at a time
+};
+
+template <class F, int... K>
+__device__ __forceinline__ void static_for_impl(F f, std::integer_sequence<int, K...>) {
+  (f(std::integral_constant<int, K>{}), ...);
+}
+template <int N, class F>
+__device__ __forceinline__ void static_for(F f) {
+  static_for_impl(f, std::make_integer_sequence<int, N>{});
+}
+
+// B or C of a tile for the four states of a wave: register i of a lane holds token
+// 4 i + (lane % 16) / 4, state lane % 4, so that token 4 i + k's state n is lane
+// 4 k + n of every row of 16, which a DPP operand broadcasts.
+template <typename T>
+struct SsmVec {
+  uint32_t w[4];
+  __device__ __forceinline__ void load(const T* base, int rows, int pitch, int N, int n0, int lane) {
+    const rsrc_t r = open_rsrc(base);
+    const int n = n0 + (lane & 3);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int t = 4 * i + ((lane & 15) >> 2);
+      const uint32_t at = t < rows && n < N ? (uint32_t)(t * pitch + n) * (uint32_t)sizeof(T) : OOB;
+      if constexpr (IS_BF16<T>) w[i] = __builtin_amdgcn_raw_buffer_load_b16(r, at, 0, 0);
+      else w[i] = __builtin_amdgcn_raw_buffer_load_b32(r, at, 0, 0);
+    }
+  }
+  __device__ __forceinline__ float at(int i) const {
+    return __builtin_bit_cast(float, IS_BF16<T> ? w[i] << 16 : w[i]);
+  }
+};
+
+// y[t] += sum_n v(4 t + n) h[t][n], v(k) lane k of a row of 16: the compiler folds the
+// broadcast into a product but not into a multiply-add, so these are written out, behind
+// the two wait states that a DPP operand asks for after its register was written.
+__device__ __forceinline__ void ssm_dots(f32x4& y, float v, const float (&h)[4][4]) {
+  float y0 = y[0], y1 = y[1], y2 = y[2], y3 = y[3];
+#define LZ_DOT(t, k, n) \
+  "v_fmac_f32_dpp %" #t ", %4, %" #n " row_newbcast:" #k " row_mask:0xf bank_mask:0xf\n"
+  asm("s_nop 1\n"
+      LZ_DOT(0, 0, 5) LZ_DOT(1, 4, 9) LZ_DOT(2, 8, 13) LZ_DOT(3, 12, 17)
+      LZ_DOT(0, 1, 6) LZ_DOT(1, 5, 10) LZ_DOT(2, 9, 14) LZ_DOT(3, 13, 18)
+      LZ_DOT(0, 2, 7) LZ_DOT(1, 6, 11) LZ_DOT(2, 10, 15) LZ_DOT(3, 14, 19)
+      LZ_DOT(0, 3, 8) LZ_DOT(1, 7, 12) LZ_DOT(2, 11, 16) LZ_DOT(3, 15, 20)
+      : "+&v"(y0), "+&v"(y1), "+&v"(y2), "+&v"(y3)
+      : "v"(v), "v"(h[0][0]), "v"(h[0][1]), "v"(h[0][2]), "v"(h[0][3]), "v"(h[1][0]),
+        "v"(h[1][1]), "v"(h[1][2]), "v"(h[1][3]), "v"(h[2][0]), "v"(h[2][1]), "v"(h[2][2]),
+        "v"(h[2][3]), "v"(h[3][0]), "v"(h[3][1]), "v"(h[3][2]), "v"(h[3][3]));
+#undef LZ_DOT
+  y = f32x4{y0, y1, y2, y3};
+}
+
+// Where a workgroup works
+struct SsmPlace {
+  int b, s, blk, g, c0, cols;   // sequence, segment, block; group, first channel, channels
+  int len, tile0, tile1;        // the sequence's length, the segment's tiles
+  __device__ __forceinline__ SsmPlace(const Ssm& p, int segments) {
+    const int nblk = p.G * p.gblocks;
+    int i = blockIdx.x;
+    blk = i % nblk;
+    i /= nblk;
+    s = i % segments;
+    b = i / segments;
+    g = blk / p.gblocks;
+    const int first = (blk - g * p.gblocks) * SSM_CH;
+    c0 = g * p.Eg + first;
+    cols = min(SSM_CH, p.Eg - first);
+    len = p.lengths ? max(0, min(p.L, p.lengths[b])) : p.L;
+    tile0 = s * p.seg_tiles;
+    tile1 = min(p.tiles, tile0 + p.seg_tiles);
+  }
+};
+
+inline int ssm_waves(int N) { return N <= 4 ? 1 : N <= 8 ? 2 : N <= 16 ? 4 : 8; }
+inline int ssm_passes(int N) { return N <= 32 ? 1 : 2; }
+
+int ssm_segments(int batch, int G, int Eg, int N, int L, bool backward);
+hipError_t launch_ssm_fwd(const Ssm& p, bool is_bf16, bool vec, hipStream_t st);
+hipError_t launch_ssm_step(const Ssm& p, float* state, bool is_bf16, hipStream_t st);
+hipError_t launch_ssm_bwd(const Ssm& p, const SsmGrad& g, void* dB, void* dC, float* dA,
+                          float* dD, float* dbias, bool is_bf16, bool vec, hipStream_t st);
+
+}  // namespace lz

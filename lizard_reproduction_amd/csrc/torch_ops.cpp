@@ -13,55 +13,12 @@
 // 35 us: gla 138 -> 87 us, swa 120 -> 75 us; a short forward (H = 4, L = 256) 17.6 ->
 // 11.4 us (10.0 since its walks fold the segment records); a decode step of the layer
 // (B = 4, hidden 2048) 201 -> 132 us with torch's projections, 48 us with rows.hip's.
-#include <c10/hip/HIPStream.h>
-#include <torch/extension.h>
-
 #include <cmath>
-#include <stdexcept>
-#include <string>
 #include <tuple>
 
-#include "../../include/lizard_hip.h"
+#include "torch_common.hpp"
 
 namespace {
-
-using at::Tensor;
-using torch::autograd::AutogradContext;
-using torch::autograd::variable_list;
-
-void* stream_of(const Tensor& t) {
-  return c10::hip::getCurrentHIPStream(t.device().index()).stream();
-}
-
-void check(int rc, const char* what) {
-  if (rc != 0)
-    throw std::runtime_error(std::string(what) + " failed (status " + std::to_string(rc) +
-                             "): " + lz_last_error());
-}
-
-template <typename T = void>
-T* ptr(const Tensor& t) {
-  return t.defined() && t.numel() ? static_cast<T*>(t.data_ptr()) : nullptr;
-}
-
-Tensor as(const Tensor& t, at::ScalarType dtype) {
-  return (t.scalar_type() == dtype ? t : t.to(dtype)).contiguous();
-}
-Tensor bf16(const Tensor& t) { return as(t, at::kBFloat16); }
-Tensor f32(const Tensor& t) { return as(t, at::kFloat); }
-
-Tensor bytes(size_t n, const Tensor& like) {
-  return at::empty({static_cast<int64_t>(n)}, like.options().dtype(at::kByte));
-}
-
-int i32(int64_t x) { return static_cast<int>(x); }
-
-bool any_grad(std::initializer_list<const Tensor*> tensors) {
-  if (!at::GradMode::is_enabled()) return false;
-  for (const Tensor* t : tensors)
-    if (t->requires_grad()) return true;
-  return false;
-}
 
 // gradients come back in the inputs' dtypes; the kernels write bf16 ones when
 // q, k and v (fq, fk and v) are all bf16, else fp32
@@ -383,4 +340,5 @@ PYBIND11_MODULE(lizard_torch, m) {
   m.def("layer_step_rows", &layer_step_rows, nogil);
   m.def("rows_linear", &rows_linear, nogil);
   m.attr("ROWS_MAX") = LZ_ROWS_MAX;
+  bind_mixers(m);
 }

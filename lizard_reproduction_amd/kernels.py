@@ -6,6 +6,10 @@ Drop-in for the reference's ``kernels`` package (``src/kernels/__init__.py``):
 * ``swa(q, k, v, meta, window, fwd_blocks=(64, 64), bwd_blocks=(64, 64))``
   -- ``src/kernels/swa.py:182-183``
 
+and, beside gla, a recurrent mixer whose decay is its own per channel and state
+entry, with what stands around it (no counterpart in the reference; conventions
+below): ``ssm``, ``short_conv``, ``group_norm``.
+
 Same signatures, shapes and conventions: tensors are ``[B, H, L, .]``; inputs
 of any float dtype are cast to bf16; outputs are bf16; gradients come back in
 each input's dtype; the gate is ``[B, L]`` (one per token, shared by heads) or
@@ -559,3 +563,276 @@ def swa(q, k, v, meta, window, fwd_blocks=FWD_BLOCKS, bwd_blocks=BWD_BLOCKS):
         # nothing to differentiate: the forward launch without the autograd node
         return _swa_fwd_launch(_bf16(q), _bf16(k), _bf16(v), _f32(meta), window)[0]
     return _SWA.apply(q, k, v, meta, window, tuple(fwd_blocks), tuple(bwd_blocks))
+
+
+# ---------------------------------------------------------------------------
+# recurrent mixers with a decay per channel and state: short causal
+# convolution, selective state space scan, group norm
+# ---------------------------------------------------------------------------
+#
+# Channels last, [B, L, channels].  Activations are bf16 or fp32; a call whose
+# activations are all bf16 reads and writes bf16, any other computes in fp32;
+# sums, states and parameters are fp32 either way.  Outputs come in x's dtype,
+# gradients in each input's.  Slices of wider rows (one projection's halves)
+# are read where they lie.
+
+_ACTIVATIONS = (torch.bfloat16, torch.float32)
+# limits of the C ABI (include/lizard_hip.h)
+CONV_MAX_TAPS, SSM_MAX_STATE, NORM_MAX_WIDTH = 4, 64, 8192
+
+
+def _require_eager(what):
+    if not _ops.plain():
+        raise RuntimeError(f"{what}: not supported under torch.func transforms or torch.jit tracing")
+
+
+def _check_activations(what, **tensors):
+    """dtypes and devices of a call's activations (z and gate may be None); the
+    first one names the device."""
+    device = None
+    for name, t in tensors.items():
+        if t is None and name in ("z", "gate"):
+            continue
+        if not isinstance(t, torch.Tensor):
+            raise ValueError(f"{what}: {name} must be a tensor, got {type(t).__name__}")
+        device = device or t.device
+        if t.device != device:
+            raise ValueError(f"{what}: {name} is on {t.device}, the others on {device}")
+        if t.dtype not in _ACTIVATIONS:
+            raise ValueError(f"{what}: {name} must be bf16 or fp32, got {t.dtype}")
+        if t.numel() >= 2 ** 40 or any(n >= 2 ** 31 for n in t.shape):
+            raise ValueError(f"{what}: {name} {tuple(t.shape)} is too large")
+    return device
+
+
+def _check_shape(what, name, t, shape):
+    if t is not None and tuple(t.shape) != tuple(shape):
+        raise ValueError(f"{what}: {name} must be {tuple(shape)}, got {tuple(t.shape)}")
+
+
+def _check_params(what, device, **params):
+    for name, (t, shape) in params.items():
+        if t is None:
+            continue
+        if not isinstance(t, torch.Tensor) or not t.is_floating_point():
+            raise ValueError(f"{what}: {name} must be a floating-point tensor")
+        if t.device != device:
+            raise ValueError(f"{what}: {name} is on {t.device}, x on {device}")
+        _check_shape(what, name, t, shape)
+
+
+def _check_lengths(what, lengths, batch, device):
+    if lengths is None:
+        return
+    if not isinstance(lengths, torch.Tensor) or lengths.dtype not in (torch.int32, torch.int64):
+        raise ValueError(f"{what}: lengths must be an int32 or int64 tensor")
+    if tuple(lengths.shape) != (batch,) or lengths.device != device:
+        raise ValueError(f"{what}: lengths must be [{batch}] on {device}, got "
+                         f"{tuple(lengths.shape)} on {lengths.device}")
+
+
+def _check_state(what, state, shape, dtype, device, in_place=False):
+    """A recurrent state; one that is updated in place has to be its own
+    memory throughout (contiguous)."""
+    if not isinstance(state, torch.Tensor) or tuple(state.shape) != tuple(shape) or \
+            state.dtype != dtype or state.device != device or \
+            (in_place and not state.is_contiguous()):
+        got = (f"{tuple(state.shape)} {state.dtype} on {state.device}"
+               if isinstance(state, torch.Tensor) else type(state).__name__)
+        raise ValueError(f"{what}: state must be {'contiguous ' if in_place else ''}{dtype} "
+                         f"{tuple(shape)} on {device}, got {got}")
+    if in_place and state.requires_grad and torch.is_grad_enabled():
+        raise ValueError(f"{what}: state is updated in place and may not require gradients")
+
+
+def _silu(what, activation):
+    if activation not in (None, "silu"):
+        raise ValueError(f"{what}: activation must be 'silu' or None, got {activation!r}")
+    return activation == "silu"
+
+
+# --- short causal convolution -------------------------------------------------
+
+def _check_conv(what, x, weight, bias, activation, dims):
+    device = _check_activations(what, x=x)
+    if x.dim() != dims or x.shape[-1] < 1:
+        raise ValueError(f"{what}: x must be {'[B, L, C]' if dims == 3 else '[B, C]'}, got "
+                         f"{tuple(x.shape)}")
+    channels = x.shape[-1]
+    if not isinstance(weight, torch.Tensor) or weight.dim() != 2 or weight.shape[0] != channels or \
+            not 1 <= weight.shape[1] <= CONV_MAX_TAPS:
+        got = tuple(weight.shape) if isinstance(weight, torch.Tensor) else type(weight).__name__
+        raise ValueError(f"{what}: weight must be [{channels}, K] with K in [1, {CONV_MAX_TAPS}], "
+                         f"got {got}")
+    _check_params(what, device, weight=(weight, weight.shape), bias=(bias, (channels,)))
+    silu = _silu(what, activation)
+    _require_gpu(x)
+    _require_eager(what)
+    return silu
+
+
+def short_conv(x, weight, bias=None, activation="silu"):
+    """Short causal convolution over the tokens of each channel:
+    y_t = act(bias + sum_j weight[:, j] x_{t-K+1+j}), rows before the first
+    being zeros.  x ``[B, L, C]``, weight ``[C, K]`` (K at most 4), bias
+    ``[C]``; activation ``"silu"`` or None.  Returns ``[B, L, C]``."""
+    silu = _check_conv("short_conv", x, weight, bias, activation, 3)
+    return _ops.load().short_conv(x, weight, bias, silu)
+
+
+def short_conv_prefill(x, weight, bias=None, activation="silu", state=None, lengths=None):
+    """``short_conv`` (no autograd) that also returns the rows a next token's
+    convolution needs, ``(y, state)``, state ``[B, K - 1, C]`` in x's dtype.
+    ``state`` is what an earlier call returned (a prompt taken in pieces),
+    None for an empty prefix; it is not written.  ``lengths`` (int ``[B]``)
+    are the lengths of a padded batch's sequences, taken into [0, L]: y past
+    them is zero, the state that after them."""
+    what = "short_conv_prefill"
+    silu = _check_conv(what, x, weight, bias, activation, 3)
+    b, length, channels = x.shape
+    shape = (b, weight.shape[1] - 1, channels)
+    if state is not None:
+        _check_state(what, state, shape, x.dtype, x.device)
+    _check_lengths(what, lengths, b, x.device)
+    if not x.numel():
+        return x.new_empty(x.shape), (x.new_zeros(shape) if state is None else state.clone())
+    return _ops.load().short_conv_prefill(x, weight, bias, silu, state, lengths)
+
+
+def short_conv_decode_step(x, weight, state, bias=None, activation="silu"):
+    """One token of each sequence, ``x [B, C]``: returns y ``[B, C]`` and moves
+    ``state`` (``[B, K - 1, C]`` in x's dtype, from ``short_conv_prefill`` or
+    zeros) on by it, in place.  No autograd."""
+    what = "short_conv_decode_step"
+    silu = _check_conv(what, x, weight, bias, activation, 2)
+    _check_state(what, state, (x.shape[0], weight.shape[1] - 1, x.shape[1]), x.dtype, x.device, True)
+    return _ops.load().short_conv_step(x[:, None], weight, state, bias, silu)[:, 0]
+
+
+# --- selective state space scan -------------------------------------------------
+
+def _check_ssm(what, x, dt, A, B, C, D, z, dt_bias, step):
+    """Checks; returns B and C as [B, L, G, N] ([B, G, N] for a step)."""
+    device = _check_activations(what, x=x, dt=dt, B=B, C=C, z=z)
+    dims = 2 if step else 3
+    form = "[B, E]" if step else "[B, L, E]"
+    if x.dim() != dims or x.shape[-1] < 1:
+        raise ValueError(f"{what}: x must be {form}, got {tuple(x.shape)}")
+    for name, t in (("dt", dt), ("z", z)):
+        _check_shape(what, name, t, x.shape)
+    lead, channels = tuple(x.shape[:-1]), x.shape[-1]
+    if not isinstance(A, torch.Tensor) or A.dim() != 2 or A.shape[0] != channels or \
+            not 1 <= A.shape[1] <= SSM_MAX_STATE:
+        got = tuple(A.shape) if isinstance(A, torch.Tensor) else type(A).__name__
+        raise ValueError(f"{what}: A must be [{channels}, N] with N in [1, {SSM_MAX_STATE}], got "
+                         f"{got}")
+    _check_params(what, device, A=(A, A.shape), D=(D, (channels,)), dt_bias=(dt_bias, (channels,)))
+    n = A.shape[1]
+    if B.dim() == dims and C.dim() == dims:
+        B, C = B.unsqueeze(-2), C.unsqueeze(-2)
+    groups = B.shape[-2] if B.dim() == dims + 1 else 0
+    if groups < 1 or channels % groups or tuple(B.shape) != (*lead, groups, n) or \
+            tuple(C.shape) != tuple(B.shape):
+        raise ValueError(f"{what}: B and C must be {form[:-4]}, N] or {form[:-4]}, G, N] with N = "
+                         f"{n} and G dividing {channels}, got {tuple(B.shape)} and "
+                         f"{tuple(C.shape)}")
+    _require_gpu(x)
+    _require_eager(what)
+    return B, C
+
+
+def ssm(x, dt, A, B, C, D=None, z=None, dt_bias=None, dt_softplus=True):
+    """Selective state space scan.  For each channel e, from a zero state,
+
+        delta_t = softplus(dt_t + dt_bias)    (without softplus: dt_t + dt_bias)
+        h_t[n]  = exp(delta_t A[e, n]) h_{t-1}[n] + delta_t x_t B_t[n]
+        y_t     = (sum_n C_t[n] h_t[n] + D x_t) silu(z_t)
+
+    x, dt, z ``[B, L, E]``; A ``[E, N]`` (N at most 64), D, dt_bias ``[E]``; B, C
+    ``[B, L, N]``, or ``[B, L, G, N]`` with E / G consecutive channels to each of
+    the G.  Returns y ``[B, L, E]``.  The backward reads states that the
+    forward keeps, one every 16 tokens (N / 4 bytes a token and channel)."""
+    B, C = _check_ssm("ssm", x, dt, A, B, C, D, z, dt_bias, False)
+    return _ops.load().ssm(x, dt, A, B, C, D, z, dt_bias, bool(dt_softplus))
+
+
+def ssm_prefill(x, dt, A, B, C, D=None, z=None, dt_bias=None, dt_softplus=True, state=None,
+                lengths=None):
+    """``ssm`` (no autograd) from ``state`` (fp32 ``[B, E, N]``, None: zeros;
+    not written) that also returns the state after the last token, for
+    ``ssm_decode_step``: ``(y, state)``.  ``lengths`` as in
+    ``short_conv_prefill``."""
+    what = "ssm_prefill"
+    B, C = _check_ssm(what, x, dt, A, B, C, D, z, dt_bias, False)
+    shape = (x.shape[0], x.shape[2], A.shape[1])
+    if state is not None:
+        _check_state(what, state, shape, torch.float32, x.device)
+    _check_lengths(what, lengths, x.shape[0], x.device)
+    if not x.numel():
+        return x.new_empty(x.shape), (x.new_zeros(shape, dtype=torch.float32)
+                                      if state is None else state.clone())
+    return _ops.load().ssm_prefill(x, dt, A, B, C, D, z, dt_bias, bool(dt_softplus), state, lengths)
+
+
+def ssm_decode_step(x, dt, A, B, C, state, D=None, z=None, dt_bias=None, dt_softplus=True):
+    """One token of each sequence on the recurrence of ``ssm``, updating
+    ``state`` (contiguous fp32 ``[B, E, N]``) in place.  x, dt, z ``[B, E]``;
+    B, C ``[B, N]`` or ``[B, G, N]``.  Returns y ``[B, E]``; no autograd."""
+    what = "ssm_decode_step"
+    B, C = _check_ssm(what, x, dt, A, B, C, D, z, dt_bias, True)
+    _check_state(what, state, (x.shape[0], x.shape[1], A.shape[1]), torch.float32, x.device, True)
+    if z is not None:
+        z = z[:, None]
+    return _ops.load().ssm_step(x[:, None], dt[:, None], A, B[:, None], C[:, None], state, D, z,
+                                dt_bias, bool(dt_softplus))[:, 0]
+
+
+# --- group norm -------------------------------------------------------------------
+
+def group_norm(x, groups, weight=None, bias=None, gate=None, activation="silu", eps=1e-5):
+    """Normalisation of each token's groups of channels (a mixer's heads):
+
+        n = (x - mean) / sqrt(var + eps) over the group,  o = n weight + bias,
+        y = act(o), or with a gate  y = o act(gate)
+
+    x ``[..., C]`` with ``groups`` dividing C, or, with ``groups=None``,
+    ``[..., G, W]`` whose last two dimensions are the groups and their channels
+    and may lie apart (``kernels.gla(...)``'s ``[B, H, L, D]`` as
+    ``y.transpose(1, 2)``).  weight, bias ``[C]``; gate of x's shape;
+    activation ``"silu"`` or None.  Returns x's shape, contiguous.  Groups have at
+    most 8192 channels.  Statistics are each token's own, so the operator is
+    causal."""
+    what = "group_norm"
+    device = _check_activations(what, x=x, gate=gate)
+    apart = groups is None
+    if apart:
+        if x.dim() < 2:
+            raise ValueError(f"{what}: x must be [..., G, W], got {tuple(x.shape)}")
+        groups, width = x.shape[-2:]
+    else:
+        if not isinstance(groups, int) or groups < 1 or x.dim() < 1 or x.shape[-1] % groups:
+            raise ValueError(f"{what}: groups must be a positive int dividing the channels of "
+                             f"{tuple(x.shape)}, got {groups!r}")
+        width = x.shape[-1] // groups
+    if groups < 1 or not 1 <= width <= NORM_MAX_WIDTH:
+        raise ValueError(f"{what}: groups of 1 to {NORM_MAX_WIDTH} channels expected, got {width} "
+                         f"in {groups} groups")
+    _check_shape(what, "gate", gate, x.shape)
+    channels = groups * width
+    _check_params(what, device, weight=(weight, (channels,)), bias=(bias, (channels,)))
+    silu = _silu(what, activation)
+    if not isinstance(eps, (int, float)) or not 0 <= eps < math.inf:
+        raise ValueError(f"{what}: eps must be a non-negative number, got {eps!r}")
+    _require_gpu(x)
+    _require_eager(what)
+
+    def split(t):   # [B, L, G, W]
+        if t is None:
+            return None
+        if not apart:
+            t = t.unflatten(-1, (groups, width))
+        while t.dim() < 4:
+            t = t[None]
+        return t if t.dim() == 4 else t.flatten(0, t.dim() - 4)
+    y = _ops.load().group_norm(split(x), weight, bias, split(gate), silu, float(eps))
+    return y.view(x.shape)

@@ -1,0 +1,629 @@
+"""The recurrent mixers' operators on the GPU against plain float64 forms
+(tests/mixers_reference.py), at the sizes, layouts and masks where they can go wrong.
+
+Tolerances count roundings: half a step of the output's type, and ``rounds`` roundings of
+fp32 of a magnitude made of absolute terms.  A term of the scan passes, a token, the decay's
+product and exponential and the state's multiply-add (4), for at most L tokens each way, then
+sums over states, channels, tokens and their workgroups' shares: 8 L + 256.  The convolution's
+and the norm's sums are at most their tokens (or channels) long, and a sigmoid is 8."""
+import pytest
+import torch
+
+from lizard_reproduction_amd import _lib, kernels
+from tests import mixers_reference as ref
+from tests.mixers_reference import check
+
+pytestmark = pytest.mark.gpu
+
+BF16, FP32 = torch.bfloat16, torch.float32
+
+
+def _gen(seed):
+    return torch.Generator().manual_seed(seed)
+
+
+def _randn(g, *shape, dtype=FP32, scale=1.0):
+    return (scale * torch.randn(shape, generator=g)).to(dtype)
+
+
+def _cuda(t):
+    return t.cuda() if isinstance(t, torch.Tensor) else t
+
+
+def _layout(t, form):
+    """The same values on the GPU in another layout."""
+    if t is None:
+        return None
+    t = t.cuda()
+    if form == "slice":       # the middle columns of a wider row, odd offset
+        wide = torch.empty(*t.shape[:-1], t.shape[-1] + 11, device="cuda", dtype=t.dtype).fill_(float("nan"))
+        wide[..., 3:3 + t.shape[-1]] = t
+        return wide[..., 3:3 + t.shape[-1]]
+    if form == "half":        # half of a row twice as wide, aligned
+        wide = torch.empty(*t.shape[:-1], 2 * t.shape[-1], device="cuda", dtype=t.dtype).fill_(float("nan"))
+        wide[..., t.shape[-1]:] = t
+        return wide[..., t.shape[-1]:]
+    if form == "swapped":     # tokens before sequences in memory
+        return t.transpose(0, 1).contiguous().transpose(0, 1)
+    if form == "strided":     # channels apart
+        wide = torch.empty(*t.shape[:-1], 2 * t.shape[-1], device="cuda", dtype=t.dtype).fill_(float("nan"))
+        wide[..., ::2] = t
+        return wide[..., ::2]
+    return t
+
+
+def _backward(y, leaves, dy):
+    names = [k for k, v in leaves.items() if v is not None]
+    return dict(zip(names, torch.autograd.grad(y, [leaves[k] for k in names], dy)))
+
+
+# --- selective state space scan ------------------------------------------------------
+
+def _ssm_inputs(b, length, e, n, groups=1, dtype=FP32, z=True, d=True, bias=True, seed=0):
+    g = _gen(seed)
+    c = dict(x=_randn(g, b, length, e, dtype=dtype), dt=_randn(g, b, length, e, dtype=dtype),
+             A=-torch.rand(e, n, generator=g) * 4 - 0.01,
+             B=_randn(g, b, length, groups, n, dtype=dtype),
+             C=_randn(g, b, length, groups, n, dtype=dtype),
+             D=_randn(g, e) if d else None, z=_randn(g, b, length, e, dtype=dtype) if z else None,
+             dt_bias=_randn(g, e) - 1 if bias else None)
+    return c, _randn(g, b, length, e, dtype=dtype)
+
+
+def _check_ssm(c, dy, form="whole", softplus=True, label=""):
+    leaves = {k: None if v is None else _layout(v, form if v.dim() > 2 else "whole").requires_grad_()
+              for k, v in c.items()}
+    y = kernels.ssm(**leaves, dt_softplus=softplus)
+    grads = _backward(y, leaves, dy.cuda())
+    want = ref.ssm(**c, softplus=softplus, dy=dy)
+    rounds = 8 * c["x"].shape[1] + 256
+    assert y.dtype == c["x"].dtype and y.is_contiguous()
+    check(y, *want["y"], rounds, f"{label} y")
+    for k, grad in grads.items():
+        assert grad.dtype == c[k].dtype
+        check(grad, *want["d" + k], rounds, f"{label} d{k}")
+    with torch.no_grad():
+        assert torch.equal(kernels.ssm(**leaves, dt_softplus=softplus), y)
+    return y, grads
+
+
+@pytest.mark.parametrize("dtype", [BF16, FP32])
+@pytest.mark.parametrize("length", [1, 2, 15, 16, 17, 33, 130])
+def test_ssm_lengths(length, dtype):
+    _check_ssm(*_ssm_inputs(2, length, 72, 16, dtype=dtype), label=f"ssm L={length}")
+
+
+@pytest.mark.parametrize("n", [1, 3, 4, 5, 8, 9, 16, 17, 24, 32, 33, 47, 64])
+def test_ssm_states(n):
+    _check_ssm(*_ssm_inputs(1, 21, 72, n, dtype=BF16 if n % 2 else FP32, seed=n), label=f"ssm N={n}")
+
+
+@pytest.mark.parametrize("e, groups", [(1, 1), (3, 3), (63, 1), (65, 1), (130, 2), (192, 3), (8, 2)])
+@pytest.mark.parametrize("dtype", [BF16, FP32])
+def test_ssm_channels_and_groups(e, groups, dtype):
+    for n in (2, 6, 16, 20):
+        _check_ssm(*_ssm_inputs(2, 19, e, n, groups, dtype=dtype, seed=e),
+                   label=f"ssm E={e} G={groups} N={n}")
+
+
+@pytest.mark.parametrize("form", ["slice", "half", "swapped", "strided"])
+@pytest.mark.parametrize("dtype", [BF16, FP32])
+def test_ssm_layouts(form, dtype):
+    c, dy = _ssm_inputs(3, 37, 64, 16, 2, dtype=dtype)
+    plain, grads = _check_ssm(c, dy, label="ssm whole")
+    y, more = _check_ssm(c, dy, form, label=f"ssm {form}")
+    assert torch.equal(plain, y)
+    for k in grads:
+        assert torch.equal(grads[k], more[k]), k
+
+
+@pytest.mark.parametrize("z, d, bias, softplus", [(False, True, True, True), (True, False, False, True),
+                                                  (False, False, False, False), (True, True, True, False)])
+def test_ssm_optional_operands(z, d, bias, softplus):
+    c, dy = _ssm_inputs(2, 35, 40, 16, z=z, d=d, bias=bias)
+    if not softplus:      # steps as they are: small and positive
+        c["dt"] = c["dt"].abs() * 0.1
+        if bias:
+            c["dt_bias"] = c["dt_bias"].abs() * 0.1
+    _check_ssm(c, dy, softplus=softplus, label="ssm optional")
+
+
+@pytest.mark.parametrize("length, e, n, dtype", [(700, 40, 16, FP32), (1030, 64, 4, BF16),
+                                                 (513, 70, 33, FP32), (900, 8, 20, BF16)])
+def test_ssm_segments(length, e, n, dtype):
+    """Few channels, long sequences: the walk is split, forward and back."""
+    lib = _lib.load()
+    assert lib.lz_ssm_fwd_workspace_bytes(1, length, e, n, 1) > 0
+    c, dy = _ssm_inputs(1, length, e, n, dtype=dtype, seed=length)
+    c["dt_bias"] = c["dt_bias"] - 3      # slow decays: the segments' states matter
+    _check_ssm(c, dy, label=f"ssm segments L={length}")
+
+
+def test_ssm_mixed_types():
+    """An fp32 operand among bf16 ones: computed in fp32, returned in x's type."""
+    c, dy = _ssm_inputs(2, 20, 48, 16, dtype=BF16)
+    c["dt"] = c["dt"].float() + 0.001
+    c["A"] = c["A"].to(BF16)
+    _check_ssm(c, dy, label="ssm mixed")
+
+
+def test_ssm_strong_and_vanishing_decays():
+    """Steps from 1e-6 to 50: states that forget at once, and that never do."""
+    c, dy = _ssm_inputs(2, 64, 64, 16)
+    g = _gen(9)
+    c["dt"] = torch.empty(2, 64, 64).uniform_(-14, 50, generator=g)
+    _check_ssm(c, dy, label="ssm decays")
+
+
+def test_ssm_gradient_is_a_difference():
+    """Central differences of the kernel's own forward along a direction, h = 2^-6: the
+    rounding of the two ends is at most rounds * 2^-24 of the output's magnitude over h, and
+    the truncation a quarter of what h and 2 h differ by (h^2 against 4 h^2), doubled."""
+    c, dy = _ssm_inputs(1, 40, 64, 16)
+    leaves = {k: v.cuda().requires_grad_() for k, v in c.items()}
+    grads = _backward(kernels.ssm(**leaves), leaves, dy.cuda())
+    mag = (ref.ssm(**c)["y"][1] * dy.double().abs()).sum().item()
+    g = _gen(5)
+    for k in c:
+        v = _randn(g, *c[k].shape)
+
+        def slope(h):
+            ends = [(kernels.ssm(**{m: (c[m] + s * h * v if m == k else c[m]).cuda() for m in c}).double()
+                     * dy.cuda()).sum().item() for s in (1, -1)]
+            return (ends[0] - ends[1]) / (2 * h)
+        h = 2.0 ** -6
+        one, two = slope(h), slope(2 * h)
+        got = (grads[k].double().cpu() * v).sum().item()
+        assert abs(got - one) <= abs(two - one) + 2 * 576 * 2.0 ** -24 * mag / h, (k, got, one, two)
+
+
+@pytest.mark.parametrize("dtype", [BF16, FP32])
+def test_ssm_prefill_in_pieces_and_steps(dtype):
+    """A prompt at once, in pieces, and token by token: one state, one output."""
+    c, _ = _ssm_inputs(3, 50, 72, 16, 2, dtype=dtype)
+    g = _gen(2)
+    h0 = _randn(g, 3, 72, 16)
+    want = ref.ssm(**c, state=h0)
+    rounds = 8 * 50 + 256
+    gpu = {k: _cuda(v) for k, v in c.items()}
+    seq = [k for k in ("x", "dt", "z", "B", "C")]
+
+    def part(lo, hi):
+        return dict(gpu, **{k: gpu[k][:, lo:hi] for k in seq})
+    y, h = kernels.ssm_prefill(**gpu, state=h0.cuda())
+    check(y, *want["y"], rounds, "prefill y")
+    check(h, *want["state"], rounds, "prefill state")
+    h, rows = h0.cuda(), []
+    for lo, hi in ((0, 1), (1, 17), (17, 17), (17, 33), (33, 50)):
+        before = h.clone()
+        row, after = kernels.ssm_prefill(**part(lo, hi), state=h)
+        assert torch.equal(before, h)
+        rows.append(row)
+        h = after
+    check(torch.cat(rows, 1), *want["y"], rounds, "pieces y")
+    check(h, *want["state"], rounds, "pieces state")
+    h, rows = h0.cuda(), []
+    for t in range(50):
+        at = {k: gpu[k][:, t] for k in seq}
+        rows.append(kernels.ssm_decode_step(**dict(gpu, **at), state=h))
+    check(torch.stack(rows, 1), *want["y"], rounds, "steps y")
+    check(h, *want["state"], rounds, "steps state")
+
+
+def test_ssm_prefill_padded_batch():
+    """Lengths from none to all, what lies past them NaN and infinite: zeros past them, the
+    state after them, and a length past the batch's taken as the batch's."""
+    c, _ = _ssm_inputs(6, 45, 70, 16)
+    h0 = _randn(_gen(3), 6, 70, 16)
+    lengths = [0, 1, 16, 31, 45, 99]
+    for k in ("x", "dt", "z", "B", "C"):
+        for i, end in enumerate(lengths):
+            c[k][i, end:] = float("nan") if i % 2 else float("inf")
+    clean = {k: (v.nan_to_num(0, 0, 0) if v is not None else None) for k, v in c.items()}
+    want = ref.ssm(**clean, state=h0, lengths=[min(n, 45) for n in lengths])
+    for kind in (torch.int32, torch.int64):
+        y, h = kernels.ssm_prefill(**{k: _cuda(v) for k, v in c.items()}, state=h0.cuda(),
+                                   lengths=torch.tensor(lengths, dtype=kind, device="cuda"))
+        check(y, *want["y"], 8 * 45 + 256, "padded y")
+        check(h, *want["state"], 8 * 45 + 256, "padded state")
+        for i, end in enumerate(lengths):
+            assert not y[i, end:].any()
+    assert torch.equal(h[0].cpu(), h0[0])
+
+
+def test_ssm_prefill_padded_batch_in_segments():
+    """Lengths that end before, in and at segments of a split sequence."""
+    c, _ = _ssm_inputs(4, 800, 24, 8)
+    c["dt_bias"] -= 3
+    lengths = [0, 5, 401, 800]
+    want = ref.ssm(**c, lengths=lengths)
+    y, h = kernels.ssm_prefill(**{k: _cuda(v) for k, v in c.items()},
+                               lengths=torch.tensor(lengths, device="cuda"))
+    check(y, *want["y"], 8 * 800 + 256, "padded segments y")
+    check(h, *want["state"], 8 * 800 + 256, "padded segments state")
+
+
+def test_empty_calls():
+    c, _ = _ssm_inputs(2, 0, 8, 4)
+    leaves = {k: _cuda(v).requires_grad_() for k, v in c.items()}
+    y = kernels.ssm(**leaves)
+    grads = _backward(y, leaves, torch.zeros_like(y))
+    assert y.shape == (2, 0, 8) and all(not g.any() for g in grads.values())
+    h0 = torch.randn(2, 8, 4, device="cuda")
+    y, h = kernels.ssm_prefill(**{k: _cuda(v) for k, v in c.items()}, state=h0)
+    assert y.shape == (2, 0, 8) and torch.equal(h, h0) and h.data_ptr() != h0.data_ptr()
+    none = {k: (t[:0] if t.dim() > 2 else t) for k, t in leaves.items()}
+    assert kernels.ssm(**none).shape == (0, 0, 8)
+    w = torch.randn(8, 4, device="cuda", requires_grad=True)
+    x = torch.zeros(2, 0, 8, device="cuda", requires_grad=True)
+    dx, dw = torch.autograd.grad(kernels.short_conv(x, w).sum(), (x, w))
+    assert dx.shape == x.shape and not dw.any()
+    y, state = kernels.short_conv_prefill(x.detach(), w.detach())
+    assert y.shape == x.shape and state.shape == (2, 3, 8) and not state.any()
+    dx, = torch.autograd.grad(kernels.group_norm(x, 2).sum(), x)
+    assert dx.shape == x.shape
+    step = torch.zeros(0, 8, device="cuda")
+    assert kernels.short_conv_decode_step(step, w.detach(), step.new_zeros(0, 3, 8)).shape == (0, 8)
+
+
+# --- short convolution ------------------------------------------------------------------
+
+def _check_conv(b, length, c, taps, act, bias, dtype, form="whole", seed=0):
+    g = _gen(seed)
+    x, w = _randn(g, b, length, c, dtype=dtype), _randn(g, c, taps)
+    bs, dy = _randn(g, c) if bias else None, _randn(g, b, length, c, dtype=dtype)
+    leaves = dict(x=_layout(x, form).requires_grad_(), weight=w.cuda().requires_grad_(),
+                  bias=bs.cuda().requires_grad_() if bias else None)
+    y = kernels.short_conv(**leaves, activation="silu" if act else None)
+    grads = _backward(y, leaves, dy.cuda())
+    want = ref.conv(x, w, bs, act, dy)
+    label = f"conv B={b} L={length} C={c} K={taps}"
+    assert y.dtype == dtype
+    check(y, *want["y"], 32, label + " y")
+    for k, grad in grads.items():
+        check(grad, *want["d" + k], 64 + b * length, label + " d" + k)
+    with torch.no_grad():
+        assert torch.equal(kernels.short_conv(**leaves, activation="silu" if act else None), y)
+
+
+@pytest.mark.parametrize("taps", [1, 2, 3, 4])
+@pytest.mark.parametrize("length", [1, 2, 3, 7, 8, 9, 70])
+def test_conv_taps_and_lengths(taps, length):
+    for dtype in (BF16, FP32):
+        _check_conv(2, length, 24, taps, True, True, dtype, seed=taps)
+
+
+@pytest.mark.parametrize("c", [1, 7, 8, 9, 63, 512, 520, 1030])
+@pytest.mark.parametrize("act, bias", [(True, False), (False, True)])
+def test_conv_channels(c, act, bias):
+    for dtype in (BF16, FP32):
+        _check_conv(3, 41, c, 4, act, bias, dtype, seed=c)
+
+
+@pytest.mark.parametrize("form", ["slice", "half", "swapped", "strided"])
+def test_conv_layouts(form):
+    for dtype in (BF16, FP32):
+        _check_conv(3, 37, 64, 4, True, True, dtype, form)
+
+
+def test_conv_many_runs():
+    """Enough tokens for the longest runs, and a last one cut short."""
+    _check_conv(3, 2501, 136, 4, True, True, FP32)
+
+
+@pytest.mark.parametrize("taps", [1, 2, 4])
+@pytest.mark.parametrize("dtype", [BF16, FP32])
+def test_conv_prefill_pieces_steps_and_padding(taps, dtype):
+    g = _gen(taps)
+    x, w, bias = _randn(g, 4, 30, 19, dtype=dtype), _randn(g, 19, taps), _randn(g, 19)
+    s0 = _randn(g, 4, taps - 1, 19, dtype=dtype)
+    gx, gw, gb = x.cuda(), w.cuda(), bias.cuda()
+    want = ref.conv(x, w, bias, True, state=s0)
+    y, s = kernels.short_conv_prefill(gx, gw, gb, state=s0.cuda())
+    check(y, *want["y"], 32, "conv prefill")
+    assert torch.equal(s.double().cpu(), want["state"][0])
+    state, rows = s0.cuda(), []
+    for lo, hi in ((0, 1), (1, 3), (3, 3), (3, 30)):
+        row, state = kernels.short_conv_prefill(gx[:, lo:hi], gw, gb, state=state)
+        rows.append(row)
+    assert torch.equal(torch.cat(rows, 1), y) and torch.equal(state, s)
+    state, rows = s0.cuda(), []
+    for t in range(30):
+        rows.append(kernels.short_conv_decode_step(gx[:, t], gw, state, gb))
+    check(torch.stack(rows, 1), *want["y"], 32, "conv steps")
+    assert torch.equal(state, s)
+    lengths = [0, 2, 30, 31]
+    bad = x.clone()
+    for i, end in enumerate(lengths):
+        bad[i, end:] = float("nan")
+    want = ref.conv(x, w, bias, True, state=s0, lengths=lengths)
+    y, s = kernels.short_conv_prefill(bad.cuda(), gw, gb, state=s0.cuda(),
+                                      lengths=torch.tensor(lengths, device="cuda"))
+    check(y, *want["y"], 32, "conv padded")
+    assert torch.equal(s.double().cpu(), want["state"][0])
+
+
+# --- group norm ----------------------------------------------------------------------------
+
+def _check_norm(shape, groups, gate, act, affine, dtype, form="whole", apart=False, seed=0):
+    """shape: x's; apart: its last two dimensions are the groups and their channels."""
+    g = _gen(seed)
+    channels = shape[-1] * (groups if apart else 1)
+    x = _randn(g, *shape, dtype=dtype, scale=1.5) + 0.5
+    z = _randn(g, *shape, dtype=dtype) if gate else None
+    w, b = (_randn(g, channels), _randn(g, channels)) if affine else (None, None)
+    dy = _randn(g, *shape, dtype=dtype)
+    leaves = dict(x=_layout(x, form).requires_grad_(), weight=w, bias=b, gate=_layout(z, form))
+    leaves = {k: v if v is None else v.cuda().detach().requires_grad_() if k in ("weight", "bias")
+              else v.requires_grad_() for k, v in leaves.items()}
+    call = dict(activation="silu" if act else None)
+    y = kernels.group_norm(leaves["x"], None if apart else groups, leaves["weight"], leaves["bias"],
+                           leaves["gate"], **call)
+    grads = _backward(y, leaves, dy.cuda())
+    flat = [t if t is None or not apart else t.flatten(-2) for t in (x, z, dy)]
+    want = ref.norm(flat[0], groups, w, b, flat[1], act, dy=flat[2])
+    width = channels // groups
+    rows = x.numel() // channels
+    label = f"norm {shape} G={groups}"
+    assert y.shape == x.shape and y.dtype == dtype and y.is_contiguous()
+
+    def like(pair, t):
+        return tuple(v.reshape(t.shape) for v in pair)
+    # a row's sums over its width, the square root, the division and the affine map
+    check(y, *like(want["y"], y), 2 * width.bit_length() + 48 + width // 8, label + " y")
+    for k, grad in grads.items():
+        rounds = 4 * width.bit_length() + 96 + width // 4 + (rows if k in ("weight", "bias") else 0)
+        check(grad, *like(want["d" + k], grad), rounds, label + " d" + k)
+    with torch.no_grad():
+        assert torch.equal(kernels.group_norm(leaves["x"], None if apart else groups, leaves["weight"],
+                                              leaves["bias"], leaves["gate"], **call), y)
+
+
+@pytest.mark.parametrize("width", [1, 2, 7, 8, 9, 24, 64, 65, 128, 200, 512, 520, 2048, 2056, 4096, 5000, 8192])
+def test_norm_widths(width):
+    for i, dtype in enumerate((BF16, FP32)):
+        _check_norm((2, 5, 3 * width), 3, bool(i), True, True, dtype, seed=width)
+
+
+@pytest.mark.parametrize("gate, act", [(True, True), (True, False), (False, True), (False, False)])
+@pytest.mark.parametrize("affine", [True, False])
+def test_norm_forms(gate, act, affine):
+    for dtype in (BF16, FP32):
+        _check_norm((3, 11, 160), 5, gate, act, affine, dtype)
+
+
+@pytest.mark.parametrize("groups", [1, 2, 17, 32, 33, 70])
+def test_norm_groups_and_rows(groups):
+    for rows in ((1,), (1, 1), (2, 63), (2, 3, 4)):
+        _check_norm((*rows, groups * 16), groups, True, True, True, BF16, seed=groups)
+
+
+@pytest.mark.parametrize("form", ["slice", "half", "swapped", "strided"])
+def test_norm_layouts(form):
+    for dtype in (BF16, FP32):
+        _check_norm((3, 13, 96), 4, True, True, True, dtype, form)
+
+
+def test_norm_of_attention_heads():
+    """[B, H, L, D] as [B, L, H, D], where it lies."""
+    for width in (64, 20):
+        _check_norm((2, 9, 5, width), 5, True, True, True, BF16, "whole", True)
+        _check_norm((2, 9, 5, width), 5, False, False, True, FP32, "swapped", True)
+    g = _gen(0)
+    y = _randn(g, 2, 5, 9, 64, dtype=BF16).cuda()          # heads before tokens
+    got = kernels.group_norm(y.transpose(1, 2), None, activation=None)
+    want = ref.norm(y.transpose(1, 2).flatten(-2), 5, act=False)["y"]
+    check(got.flatten(-2), *want, 96, "norm heads")
+
+
+def test_norm_many_rows():
+    """More rows than workgroups: each goes through several."""
+    _check_norm((2, 9001, 16), 2, True, True, True, FP32)
+
+
+def test_norm_constant_and_offset_rows():
+    """A group whose values are all one number has the bias's output; a large mean does not
+    swamp the deviations beyond the inputs' own rounding."""
+    x = torch.full((3, 2, 64), 7.0, device="cuda")
+    b = torch.randn(64, device="cuda")
+    assert torch.equal(kernels.group_norm(x, 2, torch.ones_like(b), b, activation=None),
+                       b.expand(3, 2, 64))
+    g = _gen(1)
+    off = (_randn(g, 4, 5, 256) + 1000)
+    y = kernels.group_norm(off.cuda(), 2, activation=None)
+    check(y, *ref.norm(off, 2, act=False)["y"], 128, "norm offset")
+
+
+# --- the calls together and around them ------------------------------------------------------
+
+def _mixer(g, e, n, groups):
+    return dict(conv_w=_randn(g, e, 4, scale=0.5), conv_b=_randn(g, e, scale=0.1),
+                A=-torch.rand(e, n, generator=g) * 4 - 0.1, D=_randn(g, e),
+                dt_bias=_randn(g, e) - 2, norm_w=_randn(g, e), norm_b=_randn(g, e),
+                proj=_randn(g, e, e + 2 * groups * n, scale=e ** -0.5))
+
+
+def _project(p, h, n, groups):
+    """dt, B and C as slices of one projection of the convolved rows."""
+    e = p["A"].shape[0]
+    out = h.float() @ p["proj"]
+    dt, B, C = out.split([e, groups * n, groups * n], -1)
+    return dt, B.unflatten(-1, (groups, n)), C.unflatten(-1, (groups, n))
+
+
+def _run_mixer(p, xz, n, groups):
+    e = p["A"].shape[0]
+    h = kernels.short_conv(xz[..., :e], p["conv_w"], p["conv_b"])
+    dt, B, C = _project(p, h, n, groups)
+    y = kernels.ssm(h, dt, p["A"], B, C, D=p["D"], dt_bias=p["dt_bias"])
+    return kernels.group_norm(y, 4, p["norm_w"], p["norm_b"], gate=xz[..., e:])
+
+
+def test_mixer_trains_and_decodes():
+    """Convolution, projection, scan and gated norm as a mixer runs them: the gradients of
+    all parameters against the plain forms in float64 under autograd, then a prompt in one
+    padded batch followed by single tokens against the whole sequence."""
+    e, n, groups, b, length = 64, 16, 2, 3, 40
+    g = _gen(0)
+    p = {k: v.cuda().requires_grad_() for k, v in _mixer(g, e, n, groups).items()}
+    xz = _randn(g, b, length, 2 * e).cuda().requires_grad_()
+    dy = _randn(g, b, length, e).cuda()
+    y = _run_mixer(p, xz, n, groups)
+    got = torch.autograd.grad(y, [xz, *p.values()], dy)
+
+    q = {k: v.detach().double().requires_grad_() for k, v in p.items()}
+    wide = xz.detach().double().requires_grad_()
+    rows = torch.nn.functional.pad(wide[..., :e], (0, 0, 3, 0))
+    h = torch.nn.functional.silu(sum(q["conv_w"][:, j] * rows[:, j:j + length] for j in range(4))
+                                 + q["conv_b"])
+    out = h @ q["proj"]
+    dt, B, C = out.split([e, groups * n, groups * n], -1)
+    B, C = (t.unflatten(-1, (groups, n)).repeat_interleave(e // groups, 2) for t in (B, C))
+    delta = torch.nn.functional.softplus(dt + q["dt_bias"])
+    s, ys = 0, []
+    for t in range(length):
+        s = torch.exp(delta[:, t, :, None] * q["A"]) * s + (delta * h)[:, t, :, None] * B[:, t]
+        ys.append((s * C[:, t]).sum(-1))
+    o = torch.nn.functional.group_norm((torch.stack(ys, 1) + q["D"] * h).reshape(-1, e), 4,
+                                       q["norm_w"], q["norm_b"], 1e-5).view(b, length, e)
+    ref_y = o * torch.nn.functional.silu(wide[..., e:])
+    want = torch.autograd.grad(ref_y, [wide, *q.values()], dy.double())
+    # each of the three operators and the fp32 product is within (8 L + 256) 2^-24 of its
+    # magnitudes; the norm divides by deviations of order one: four of them, twice over
+    tol = 8 * (8 * length + 256) * 2.0 ** -24
+    for a, w in zip((y, *got), (ref_y, *want)):
+        assert (a.double() - w).norm() <= tol * w.norm()
+
+    with torch.no_grad():
+        lengths = torch.tensor([40, 1, 17], device="cuda")
+        h, conv_state = kernels.short_conv_prefill(xz[..., :e], p["conv_w"], p["conv_b"], lengths=lengths)
+        dt, B, C = _project(p, h, n, groups)
+        _, state = kernels.ssm_prefill(h, dt, p["A"], B, C, D=p["D"], dt_bias=p["dt_bias"], lengths=lengths)
+        token = _randn(g, b, 2 * e).cuda()
+        h = kernels.short_conv_decode_step(token[:, :e], p["conv_w"], conv_state, p["conv_b"])
+        dt, B, C = _project(p, h, n, groups)
+        step = kernels.ssm_decode_step(h, dt, p["A"], B, C, state, D=p["D"], dt_bias=p["dt_bias"])
+        step = kernels.group_norm(step, 4, p["norm_w"], p["norm_b"], gate=token[:, e:])
+        for i, end in enumerate(lengths.tolist()):
+            whole = torch.cat([xz[i:i + 1, :end], token[i:i + 1, None]], 1)
+            last = _run_mixer(p, whole, n, groups)[0, -1]
+            assert (step[i] - last).norm() <= tol * last.norm()
+
+
+def _calls(seed, dtype=BF16):
+    """Each operator's training call on its own operands: (call, leaves, dy)."""
+    c, dy = _ssm_inputs(2, 600, 72, 16, dtype=dtype, seed=seed)
+    g = _gen(seed + 100)
+    ssm = {k: v.cuda().requires_grad_() for k, v in c.items()}
+    conv = dict(x=_randn(g, 2, 300, 72, dtype=dtype).cuda().requires_grad_(),
+                weight=_randn(g, 72, 4).cuda().requires_grad_(), bias=_randn(g, 72).cuda().requires_grad_())
+    norm = dict(x=_randn(g, 2, 300, 64, dtype=dtype).cuda().requires_grad_(),
+                weight=_randn(g, 64).cuda().requires_grad_(), bias=_randn(g, 64).cuda().requires_grad_(),
+                gate=_randn(g, 2, 300, 64, dtype=dtype).cuda().requires_grad_())
+    return [(kernels.ssm, ssm, dy.cuda()),
+            (kernels.short_conv, conv, _randn(g, 2, 300, 72, dtype=dtype).cuda()),
+            (lambda x, **k: kernels.group_norm(x, 4, **k), norm, _randn(g, 2, 300, 64, dtype=dtype).cuda())]
+
+
+def _train(call, leaves, dy):
+    y = call(**leaves)
+    return [y, *torch.autograd.grad(y, list(leaves.values()), dy)]
+
+
+def test_repeated_and_interleaved_calls_give_the_same_bits():
+    first = [[_train(*c) for c in _calls(s)] for s in (0, 1)]
+    cases = [_calls(s) for s in (0, 1)]
+    for _ in range(3):
+        for s in (1, 0):
+            for case, want in zip(cases[s], first[s]):
+                for a, b in zip(_train(*case), want):
+                    assert torch.equal(a, b)
+
+
+def test_side_streams():
+    """Two streams at once, operands made on the default one: the same bits."""
+    cases = [_calls(s) for s in (0, 1)]
+    want = [[_train(*c) for c in cs] for cs in cases]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    got = [[], []]
+    for _ in range(4):
+        for i, stream in enumerate(streams):
+            stream.wait_stream(torch.cuda.default_stream())
+            with torch.cuda.stream(stream):
+                got[i] = [_train(*c) for c in cases[i]]
+    torch.cuda.synchronize()
+    for a, b in zip(got, want):
+        for x, y in zip(a, b):
+            for s, t in zip(x, y):
+                assert torch.equal(s, t)
+
+
+def test_some_inputs_without_gradients_and_autograd_features():
+    for call, leaves, dy in _calls(0):
+        whole = _train(call, leaves, dy)
+        for k, grad in zip(leaves, whole[1:]):
+            only = {m: v.detach().requires_grad_(m == k) for m, v in leaves.items()}
+            got, = torch.autograd.grad(call(**only), only[k], dy)
+            assert torch.equal(got, grad), k
+        packed = []
+        with torch.autograd.graph.saved_tensors_hooks(lambda t: packed.append(t) or t.cpu(),
+                                                      lambda t: t.cuda()):
+            y = call(**leaves)
+        for a, b in zip(torch.autograd.grad(y, list(leaves.values()), dy), whole[1:]):
+            assert torch.equal(a, b)
+        assert len(packed) == len(leaves)
+        with pytest.raises(RuntimeError, match="second time"):
+            torch.autograd.grad(y, list(leaves.values()), dy)
+        y = call(**leaves)
+        with torch.no_grad():
+            leaves["x"].add_(0)
+        with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+            y.sum().backward()
+        # an upstream gradient of another layout and type
+        y = call(**leaves)
+        odd = dy.transpose(0, 1).contiguous().transpose(0, 1)
+        for a, b in zip(torch.autograd.grad(y, list(leaves.values()), odd), whole[1:]):
+            assert torch.equal(a, b)
+        # gradients of gradients have no graph
+        y = call(**leaves)
+        dx, = torch.autograd.grad(y.float().sum(), leaves["x"], create_graph=True)
+        assert not dx.requires_grad or dx.grad_fn is None
+
+
+def test_capture_transforms_and_other_devices_are_refused():
+    for call, leaves, dy in _calls(0):
+        plain = {k: v.detach() for k, v in leaves.items()}
+        with pytest.raises((RuntimeError, ValueError)):
+            torch.func.vmap(lambda x: call(**dict(plain, x=x)))(plain["x"][None])
+        with torch.autograd.forward_ad.dual_level(), pytest.raises(RuntimeError):
+            x = leaves["x"]
+            call(**dict(leaves, x=torch.autograd.forward_ad.make_dual(x, torch.ones_like(x))))
+        with pytest.raises(ValueError, match="is on cpu"):
+            call(**dict(plain, **{list(plain)[1]: list(plain.values())[1].cpu()}))
+
+
+def test_capture_is_refused(monkeypatch):
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: True)
+    for call, leaves, _ in _calls(0):
+        with pytest.raises(RuntimeError, match="capture"):
+            call(**leaves)
+
+
+def test_expanded_operands_get_their_gradients():
+    """B and C shared by the sequences of a batch, one dt for all channels, x of one
+    sequence: strides of zero, gradients summed by autograd."""
+    c, dy = _ssm_inputs(3, 40, 64, 16)
+    small = dict(c, x=c["x"][:1], dt=c["dt"][..., :1], B=c["B"][:1], C=c["C"][:, :1])
+    shapes = {k: c[k].shape for k in ("x", "dt", "B", "C")}
+    leaves = {k: v.cuda().requires_grad_() for k, v in small.items()}
+    grads = _backward(kernels.ssm(**{k: v.expand(shapes[k]) if k in shapes else v
+                                     for k, v in leaves.items()}), leaves, dy.cuda())
+    whole = {k: v.expand(shapes[k]).contiguous() if k in shapes else v for k, v in small.items()}
+    want = ref.ssm(**whole, dy=dy)
+    for k, grad in grads.items():
+        value, mag = (t.double() for t in want["d" + k])
+        if k in shapes:
+            dims = [i for i, (a, b) in enumerate(zip(small[k].shape, shapes[k])) if a != b]
+            value, mag = value.sum(dims, keepdim=True), mag.sum(dims, keepdim=True)
+        check(grad, value, mag, 8 * 40 + 256 + 64, f"expanded d{k}")
