@@ -32,7 +32,7 @@ int check_ssm_sizes(const char* what, long long batch, long long length, long lo
     return fail(1, "%s: %lld channels beyond %d unsupported", what, channels, LZ_MIXER_MAX_STRIDE);
   if (batch * length > ROWS_LIMIT)
     return fail(1, "%s: %lld tokens exceed the 2^31 - 2^20 limit", what, batch * length);
-  // workgroups of up to 512 threads, 64 segments a sequence; sums of 64 outputs
+  // workgroups of up to 768 threads, 64 segments a sequence; sums of 64 outputs
   const long long blocks = groups * ((channels / groups + 63) / 64);
   if (batch * blocks > (1LL << 23) / 64 || batch > 65535)
     return fail(1, "%s: batch %lld x %lld blocks of channels exceed the grid", what, batch, blocks);
@@ -87,10 +87,9 @@ size_t ssm_records(const lz::Ssm& p) {
   return (size_t)p.batch * (p.S - 1) * p.E * (p.N + 1);
 }
 
-// Whether a thread's share of a row (SsmSplit::V channels) is whole and aligned in every row
+// Whether a thread's share of a row (SSM_V channels) is whole and aligned in every row
 bool ssm_vec(const lz::Ssm& p, bool bf16, std::initializer_list<const void*> rows) {
-  const int W = lz::ssm_waves(p.N), V = 16 / W < 8 ? 16 / W : 8, size = bf16 ? 2 : 4;
-  const int bytes = V * size < 16 ? V * size : 16;
+  const int V = lz::SSM_V, bytes = V * (bf16 ? 2 : 4);
   if (p.Eg % V) return false;
   for (long long s : {p.x_b, p.dt_b, p.z ? p.z_b : 0LL, (long long)p.x_t, (long long)p.dt_t,
                       (long long)p.z_t})
@@ -104,14 +103,17 @@ lz::Ssm ssm_sizes(int batch, int length, int channels, int state, int groups, bo
   lz_ssm_args a = {};
   a.batch = batch, a.length = length, a.channels = channels, a.state = state, a.groups = groups;
   lz::Ssm p = ssm_of(&a, false);
-  ssm_split(p, lz::ssm_segments(p.batch, p.G, p.Eg, p.N, p.L, backward));
+  ssm_split(p, lz::ssm_segments(p.batch, p.G, p.Eg, p.L, backward));
   return p;
 }
 
-int ssm_nq(const lz::Ssm& p) { return 4 * lz::ssm_waves(p.N) * lz::ssm_passes(p.N); }
-
 size_t ssm_part_bc(const lz::Ssm& p) {
-  return (size_t)p.G * p.gblocks * p.batch * p.L * 2 * ssm_nq(p);
+  return (size_t)p.G * p.gblocks * p.batch * p.L * 2 * lz::ssm_bwd_padded(p.N);
+}
+
+// Sums over n that pass from one launch to the next
+size_t ssm_acc(const lz::Ssm& p) {
+  return p.N > lz::SSM_BWD_STATES ? 3 * (size_t)p.batch * p.L * p.E : 0;
 }
 
 bool ssm_sizes_ok(int batch, int length, int channels, int state, int groups) {
@@ -137,7 +139,7 @@ extern "C" int lz_ssm_fwd(const lz_ssm_args* args, const float* state_in, float*
   if (int rc = check_ssm("ssm_fwd", args, false)) return rc;
   if (!y) return fail(1, "ssm_fwd: null output pointer");
   lz::Ssm p = ssm_of(args, false);
-  ssm_split(p, lz::ssm_segments(p.batch, p.G, p.Eg, p.N, p.L, false));
+  ssm_split(p, lz::ssm_segments(p.batch, p.G, p.Eg, p.L, false));
   const size_t need = ssm_records(p) * 4;
   if (need && (!workspace || workspace_bytes < need))
     return fail(1, "ssm_fwd: workspace of %zu bytes given, %zu needed", workspace_bytes, need);
@@ -161,7 +163,8 @@ extern "C" size_t lz_ssm_bwd_workspace_bytes(int batch, int length, int channels
                                              int groups) {
   if (!ssm_sizes_ok(batch, length, channels, state, groups)) return 0;
   const lz::Ssm p = ssm_sizes(batch, length, channels, state, groups, true);
-  return (ssm_part_bc(p) + (size_t)p.batch * p.S * p.E * (p.N + 2) + ssm_records(p)) * 4;
+  return (ssm_part_bc(p) + (size_t)p.batch * p.S * p.E * (p.N + 2) + ssm_records(p) +
+          ssm_acc(p)) * 4;
 }
 
 extern "C" int lz_ssm_bwd(const lz_ssm_args* args, const float* states, const void* dy, void* dx,
@@ -171,18 +174,21 @@ extern "C" int lz_ssm_bwd(const lz_ssm_args* args, const float* states, const vo
   if (!states || !dy || !dx || !ddt || !dB || !dC || !dA || (args->z && !dz))
     return fail(1, "ssm_bwd: null pointer");
   lz::Ssm p = ssm_of(args, false);
-  ssm_split(p, lz::ssm_segments(p.batch, p.G, p.Eg, p.N, p.L, true));
+  ssm_split(p, lz::ssm_segments(p.batch, p.G, p.Eg, p.L, true));
   const size_t need = lz_ssm_bwd_workspace_bytes(p.batch, p.L, p.E, p.N, p.G);
   if (!workspace || workspace_bytes < need)
     return fail(1, "ssm_bwd: workspace of %zu bytes given, %zu needed", workspace_bytes, need);
   p.saved = const_cast<float*>(states);
   lz::SsmGrad g = {};
   g.dy = dy, g.dx = dx, g.ddt = ddt, g.dz = dz;
-  g.part_bc = (float*)workspace;
+  g.acc = (float*)workspace;
+  g.part_bc = g.acc + ssm_acc(p);
   g.part_a = g.part_bc + ssm_part_bc(p);
   g.part_d = g.part_a + (size_t)p.batch * p.S * p.E * p.N;
   g.rec = g.part_d + (size_t)p.batch * p.S * p.E * 2;
   g.dsum = g.rec + (size_t)p.batch * (p.S - 1) * p.E * p.N;
+  g.acc_step = (long long)p.batch * p.L * p.E;
+  g.NQ = lz::ssm_bwd_padded(p.N);
   const bool vec = ssm_vec(p, args->bf16, {dy, dx, ddt, dz});
   return hip_status(lz::launch_ssm_bwd(p, g, dB, dC, dA, dD, ddt_bias, args->bf16 != 0, vec,
                                        (hipStream_t)stream), "ssm_bwd");

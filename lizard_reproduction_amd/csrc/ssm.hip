@@ -11,114 +11,132 @@
 
 namespace lz {
 
+// STATE: the segments' own states alone, without C, z and y.
 template <typename T, int W, int NP, bool VEC, bool STATE>
-__global__ __launch_bounds__(64 * W) void ssm_fwd_kernel(Ssm p) {
-  using Split = SsmSplit<W>;
-  constexpr int V = Split::V, R = Split::R;
-  __shared__ float sd[SSM_TILE], su[SSM_TILE], sy[STATE ? 1 : W * SSM_TILE];
+__global__ __launch_bounds__(64 * (W + SSM_HELPERS)) void ssm_fwd_kernel(Ssm p) {
+  constexpr int V = SSM_V;
+  // two tiles of each: one worked on by the scan waves, one by the helpers
+  __shared__ float sd[2][SSM_TILE], su[2][SSM_TILE], sy[STATE ? 1 : 2 * W][SSM_TILE];
   const int segments = STATE ? p.S - 1 : p.S;
   const SsmPlace at(p, segments);
-  const int tid = threadIdx.x, lane = tid & 63;
-  const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int c = at.c0 + lane;
-  const bool mine = lane < at.cols;
-
-  float A2[NP][4], h[NP][4];
-#pragma unroll
-  for (int q = 0; q < NP; ++q)
-#pragma unroll
-    for (int k = 0; k < 4; ++k) {
-      const int n = 4 * (w + W * q) + k;
-      const bool in = mine && n < p.N;
-      A2[q][k] = in ? p.A[(size_t)c * p.N + n] * LOG2E : 0.f;
-      h[q][k] = in && !STATE && p.state_in ? p.state_in[((size_t)at.b * p.E + c) * p.N + n] : 0.f;
-    }
-  if constexpr (!STATE) {
-    // the state before this segment, from the earlier segments' own states
-    for (int j = 0; j < at.s; ++j) {
-      const size_t rec = (size_t)at.b * (p.S - 1) + j;
-      const float d = mine ? p.dsum[rec * p.E + c] : 0.f;
-#pragma unroll
-      for (int q = 0; q < NP; ++q)
-#pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          const int n = 4 * (w + W * q) + k;
-          if (mine && n < p.N)
-            h[q][k] = fmaf(__builtin_amdgcn_exp2f(A2[q][k] * d), h[q][k],
-                           p.rec[(rec * p.N + n) * p.E + c]);
-        }
-    }
-  }
-
-  // this thread's share of a tile's rows
-  const int tr = tid / Split::COLS, tc = (tid % Split::COLS) * V, left = at.cols - tc;
-  float bias[V], D[V];
-#pragma unroll
-  for (int i = 0; i < V; ++i) {
-    bias[i] = p.bias && i < left ? p.bias[at.c0 + tc + i] : 0.f;
-    D[i] = !STATE && p.D && i < left ? p.D[at.c0 + tc + i] : 0.f;
-  }
-  // where the next tile's rows begin, and from one tile to the next
+  const int lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int E = p.E, N = p.N;
   const long long first = (long long)at.tile0 * SSM_TT;
-  const T* xb = (const T*)p.x + at.b * p.x_b + first * p.x_t + at.c0;
-  const T* db = (const T*)p.dt + at.b * p.dt_b + first * p.dt_t + at.c0;
-  const T* zb = p.z ? (const T*)p.z + at.b * p.z_b + first * p.z_t + at.c0 : nullptr;
-  const T* Bb = (const T*)p.B + at.b * p.B_b + first * p.B_t + (long long)at.g * p.B_g;
-  const T* Cb = (const T*)p.C + at.b * p.C_b + first * p.C_t + (long long)at.g * p.C_g;
-  T* yb = (T*)p.y + ((long long)at.b * p.L + first) * p.E + at.c0;
-  float* saved = p.saved ? p.saved + ((size_t)at.b * p.tiles + at.tile0) * p.N * p.E : nullptr;
-  const size_t saved_step = (size_t)p.N * p.E;
-  const int x_t = p.x_t, dt_t = p.dt_t, z_t = p.z_t, B_t = p.B_t, C_t = p.C_t, E = p.E, N = p.N;
-  const bool has_z = p.z, soft = p.softplus;
+  auto rows_of = [&](int tile) { return min(SSM_TT, at.len - tile * SSM_TT); };
 
-  RawRow<T, V, VEC> xr[R], dr[R], zr[R];
-  SsmVec<T> Bv[NP], Cv[NP];
-  auto load = [&](int rows) {
-    const rsrc_t rx = open_rsrc(xb), rd = open_rsrc(db), rz = open_rsrc(zb);
+  // --- rows to delta and u, shares of y to rows (helper) ------------------------------
+  const int tid = (int)threadIdx.x - 64 * W;
+  const int row = tid / SSM_COLS, tc = (tid % SSM_COLS) * V, left = at.cols - tc;
+  const bool has_z = p.z, soft = p.softplus;
+  const int x_t = p.x_t, dt_t = p.dt_t, z_t = p.z_t;
+  const T* xb = (const T*)p.x + at.b * p.x_b + first * x_t + at.c0;
+  const T* db = (const T*)p.dt + at.b * p.dt_b + first * dt_t + at.c0;
+  const T* zb = has_z ? (const T*)p.z + at.b * p.z_b + first * z_t + at.c0 : nullptr;
+  T* yb = (T*)p.y + ((long long)at.b * p.L + first) * E + at.c0;
+  RawRow<T, V, VEC> xr, dr, zr;   // the next tile's rows
+  float bias[V], D[V];
+  auto load_params = [&] {
 #pragma unroll
-    for (int r = 0; r < R; ++r) {
-      const int row = tr + r * Split::ROWS;
-      xr[r] = load_raw<T, V, VEC>(rx, row * x_t + tc, row < rows, left);
-      dr[r] = load_raw<T, V, VEC>(rd, row * dt_t + tc, row < rows, left);
-      if (!STATE) zr[r] = load_raw<T, V, VEC>(rz, row * z_t + tc, has_z && row < rows, left);
+    for (int i = 0; i < V; ++i) {
+      bias[i] = p.bias && i < left ? p.bias[at.c0 + tc + i] : 0.f;
+      D[i] = !STATE && p.D && i < left ? p.D[at.c0 + tc + i] : 0.f;
     }
+  };
+  auto load_rows = [&](int rows) {
+    const rsrc_t rx = open_rsrc(xb), rd = open_rsrc(db), rz = open_rsrc(zb);
+    {
+      xr = load_raw<T, V, VEC>(rx, row * x_t + tc, row < rows, left);
+      dr = load_raw<T, V, VEC>(rd, row * dt_t + tc, row < rows, left);
+      if (!STATE) zr = load_raw<T, V, VEC>(rz, row * z_t + tc, has_z && row < rows, left);
+    }
+    xb += SSM_TT * (long long)x_t;
+    db += SSM_TT * (long long)dt_t;
+    if (has_z) zb += SSM_TT * (long long)z_t;
+  };
+  auto prep = [&](int rows, int buf) {
+    {
+      float d[V], u[V];
+#pragma unroll
+      for (int i = 0; i < V; ++i) {
+        d[i] = dr.at(i) + bias[i];
+        if (soft) d[i] = softplus(d[i]);
+        if (row >= rows) d[i] = 0.f;   // past the length: the state stays as it is
+        u[i] = d[i] * xr.at(i);
+      }
+      put_row(sd[buf] + row * SSM_CH + tc, d);
+      put_row(su[buf] + row * SSM_CH + tc, u);
+    }
+  };
+  auto finish = [&](int tile, int buf, const RawRow<T, V, VEC>& x,
+                    const RawRow<T, V, VEC>& z) {
+    const int t0 = tile * SSM_TT, rows = rows_of(tile);
+    const rsrc_t ry = open_rsrc(yb);
+    {
+      float y[V];
+#pragma unroll
+      for (int i = 0; i < V; ++i) y[i] = x.at(i) * D[i];
+#pragma unroll
+      for (int j = 0; j < W; ++j) add_row(y, sy[STATE ? 0 : buf * W + j] + row * SSM_CH + tc);
+      RawRow<T, V, VEC> out;
+#pragma unroll
+      for (int i = 0; i < V; ++i) {
+        const float g = z.at(i);
+        if (has_z) y[i] *= g * sigmoid(g);
+        out.set(i, row < rows ? y[i] : 0.f);
+      }
+      store_raw<T, V, VEC>(ry, row * E + tc, row < p.L - t0, left, out);
+    }
+    yb += SSM_TT * (long long)E;
+  };
+
+  // --- the walk (scan) ------------------------------------------------------------------
+  const int w = wave, c = at.c0 + lane;
+  const bool mine = lane < at.cols;
+  const int B_t = p.B_t, C_t = p.C_t;
+  const T* Bb = (const T*)p.B + at.b * p.B_b + first * B_t + (long long)at.g * p.B_g;
+  const T* Cb = (const T*)p.C + at.b * p.C_b + first * C_t + (long long)at.g * p.C_g;
+  float* saved = p.saved ? p.saved + ((size_t)at.b * p.tiles + at.tile0) * N * E : nullptr;
+  float A2[NP][4], h[NP][4], dsum = 0.f;
+  SsmVec<T> Bv[NP], Cv[NP];
+  auto start = [&] {
+#pragma unroll
+    for (int q = 0; q < NP; ++q)
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const int n = 4 * (w + W * q) + k;
+        const bool in = mine && n < N;
+        A2[q][k] = in ? p.A[(size_t)c * N + n] * LOG2E : 0.f;
+        h[q][k] = in && !STATE && p.state_in ? p.state_in[((size_t)at.b * E + c) * N + n] : 0.f;
+      }
+    if constexpr (!STATE) {
+      // the state before this segment, from the earlier segments' own states
+      for (int j = 0; j < at.s; ++j) {
+        const size_t rec = (size_t)at.b * (p.S - 1) + j;
+        const float d = mine ? p.dsum[rec * E + c] : 0.f;
+#pragma unroll
+        for (int q = 0; q < NP; ++q)
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            const int n = 4 * (w + W * q) + k;
+            if (mine && n < N)
+              h[q][k] = fmaf(__builtin_amdgcn_exp2f(A2[q][k] * d), h[q][k],
+                             p.rec[(rec * N + n) * E + c]);
+          }
+      }
+    }
+  };
+  auto load_bc = [&](int rows) {
 #pragma unroll
     for (int q = 0; q < NP; ++q) {
       Bv[q].load(Bb, rows, B_t, N, 4 * (w + W * q), lane);
       if (!STATE) Cv[q].load(Cb, rows, C_t, N, 4 * (w + W * q), lane);
     }
-    xb += SSM_TT * (long long)x_t;
-    db += SSM_TT * (long long)dt_t;
-    if (has_z) zb += SSM_TT * (long long)z_t;
     Bb += SSM_TT * (long long)B_t;
     Cb += SSM_TT * (long long)C_t;
   };
-
-  float dsum = 0.f;
-  if (at.tile0 < at.tile1) load(min(SSM_TT, at.len - at.tile0 * SSM_TT));
-  for (int tile = at.tile0; tile < at.tile1; ++tile) {
-    const int t0 = tile * SSM_TT;
-    const int rows = min(SSM_TT, at.len - t0);
-    float xv[R][V], gate[R][V];
-#pragma unroll
-    for (int r = 0; r < R; ++r) {
-      const int row = tr + r * Split::ROWS;
-#pragma unroll
-      for (int i = 0; i < V; ++i) {
-        const float x = xr[r].at(i);
-        float d = dr[r].at(i) + bias[i];
-        if (soft) d = softplus(d);
-        if (row >= rows) d = 0.f;   // past the length: the state stays as it is
-        sd[(tc + i) * SSM_PITCH + row] = d;
-        su[(tc + i) * SSM_PITCH + row] = d * x;
-        xv[r][i] = x * D[i];
-        if (!STATE) {
-          const float z = zr[r].at(i);
-          gate[r][i] = has_z ? z * sigmoid(z) : 1.f;
-        }
-      }
-    }
-    float Bf[NP][4], Cf[NP][4];
+  float Bf[NP][4], Cf[NP][4];
+  auto take_bc = [&] {
 #pragma unroll
     for (int q = 0; q < NP; ++q)
 #pragma unroll
@@ -126,76 +144,92 @@ __global__ __launch_bounds__(64 * W) void ssm_fwd_kernel(Ssm p) {
         Bf[q][i] = Bv[q].at(i);
         if (!STATE) Cf[q][i] = Cv[q].at(i);
       }
-    if (tile + 1 < at.tile1) load(min(SSM_TT, at.len - t0 - SSM_TT));
-    if (!STATE && saved) {
+  };
+  auto save = [&] {
+    if (STATE || !saved) return;
 #pragma unroll
-      for (int q = 0; q < NP; ++q)
+    for (int q = 0; q < NP; ++q)
 #pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          const int n = 4 * (w + W * q) + k;
-          if (mine && n < N) saved[(size_t)n * E + c] = h[q][k];
-        }
-      saved += saved_step;
-    }
-    __syncthreads();
-    if (rows > 0) {
+      for (int k = 0; k < 4; ++k) {
+        const int n = 4 * (w + W * q) + k;
+        if (mine && n < N) saved[(size_t)n * E + c] = h[q][k];
+      }
+    saved += (size_t)N * E;
+  };
+  auto scan = [&](int buf) {
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const f32x4 dl = *reinterpret_cast<const f32x4*>(sd + lane * SSM_PITCH + 4 * i);
-        const f32x4 ul = *reinterpret_cast<const f32x4*>(su + lane * SSM_PITCH + 4 * i);
-        f32x4 yl = {0.f, 0.f, 0.f, 0.f};
-        if (STATE) dsum += (dl[0] + dl[1]) + (dl[2] + dl[3]);
+    for (int i = 0; i < 4; ++i) {
+      const f32x4 dl = get_tokens(sd[buf], 4 * i, lane), ul = get_tokens(su[buf], 4 * i, lane);
+      f32x4 yl = {0.f, 0.f, 0.f, 0.f};
+      if (STATE) dsum += (dl[0] + dl[1]) + (dl[2] + dl[3]);
 #pragma unroll
-        for (int q = 0; q < NP; ++q) {
-          float hs[4][4];
-          static_for<4>([&](auto kt) {
-            constexpr int t = decltype(kt)::value;
-            static_for<4>([&](auto kn) {
-              constexpr int n = decltype(kn)::value;
-              const float a = __builtin_amdgcn_exp2f(dl[t] * A2[q][n]);
-              h[q][n] = fmaf(a, h[q][n], dpp<DPP_BCAST + 4 * t + n>(Bf[q][i]) * ul[t]);
-              hs[t][n] = h[q][n];
-            });
+      for (int q = 0; q < NP; ++q) {
+        float hs[4][4];
+        static_for<4>([&](auto kt) {
+          constexpr int t = decltype(kt)::value;
+          static_for<4>([&](auto kn) {
+            constexpr int n = decltype(kn)::value;
+            const float a = __builtin_amdgcn_exp2f(dl[t] * A2[q][n]);
+            h[q][n] = fmaf(a, h[q][n], dpp<DPP_BCAST + 4 * t + n>(Bf[q][i]) * ul[t]);
+            hs[t][n] = h[q][n];
           });
-          if (!STATE) ssm_dots(yl, Cf[q][i], hs);
-        }
-        if (!STATE) *reinterpret_cast<f32x4*>(sy + w * SSM_TILE + lane * SSM_PITCH + 4 * i) = yl;
+        });
+        if (!STATE) ssm_dots(yl, Cf[q][i], hs);
       }
+      if (!STATE) put_tokens(sy[STATE ? 0 : buf * W + w], 4 * i, lane, yl);
     }
-    __syncthreads();
-    if constexpr (!STATE) {
-      const rsrc_t ry = open_rsrc(yb);
+  };
+  auto end = [&] {
+    if (!mine) return;
+    const size_t rec = (size_t)at.b * (p.S - 1) + at.s;
+    if (STATE && w == 0) p.dsum[rec * E + c] = dsum;
 #pragma unroll
-      for (int r = 0; r < R; ++r) {
-        const int row = tr + r * Split::ROWS;
-        RawRow<T, V, VEC> out;
+    for (int q = 0; q < NP; ++q)
 #pragma unroll
-        for (int i = 0; i < V; ++i) {
-          float y = xv[r][i];
-#pragma unroll
-          for (int j = 0; j < W; ++j) y += sy[j * SSM_TILE + (tc + i) * SSM_PITCH + row];
-          out.set(i, row < rows ? y * gate[r][i] : 0.f);
-        }
-        store_raw<T, V, VEC>(ry, row * E + tc, row < p.L - t0, left, out);
+      for (int k = 0; k < 4; ++k) {
+        const int n = 4 * (w + W * q) + k;
+        if (n >= N) continue;
+        if (STATE)
+          p.rec[(rec * N + n) * E + c] = h[q][k];
+        else if (p.state_out && at.s == p.S - 1)
+          p.state_out[((size_t)at.b * E + c) * N + n] = h[q][k];
       }
-      yb += SSM_TT * (long long)E;
-    }
-  }
+  };
 
-  if (!mine) return;
-  const size_t rec = (size_t)at.b * (p.S - 1) + at.s;
-  if (STATE && w == 0) p.dsum[rec * p.E + c] = dsum;
-#pragma unroll
-  for (int q = 0; q < NP; ++q)
-#pragma unroll
-    for (int k = 0; k < 4; ++k) {
-      const int n = 4 * (w + W * q) + k;
-      if (n >= p.N) continue;
-      if (STATE)
-        p.rec[(rec * p.N + n) * p.E + c] = h[q][k];
-      else if (p.state_out && at.s == p.S - 1)
-        p.state_out[((size_t)at.b * p.E + c) * p.N + n] = h[q][k];
+  const int t0 = at.tile0, t1 = at.tile1;   // t0 < t1
+  if (wave >= W) {
+    RawRow<T, V, VEC> x1, z1, x0, z0;   // of this tile and the one before
+    load_params();
+    load_rows(rows_of(t0));
+    prep(rows_of(t0), 0);
+    x1 = xr, z1 = zr;
+    if (t0 + 1 < t1) load_rows(rows_of(t0 + 1));
+    __syncthreads();
+    for (int tile = t0; tile < t1; ++tile) {
+      const int buf = (tile - t0) & 1;
+      if (!STATE && tile > t0) finish(tile - 1, buf ^ 1, x0, z0);
+      x0 = x1, z0 = z1;
+      if (tile + 1 < t1) {
+        prep(rows_of(tile + 1), buf ^ 1);
+        x1 = xr, z1 = zr;
+        if (tile + 2 < t1) load_rows(rows_of(tile + 2));
+      }
+      __syncthreads();
     }
+    if (!STATE) finish(t1 - 1, (t1 - 1 - t0) & 1, x0, z0);
+  } else {
+    load_bc(rows_of(t0));
+    start();
+    __syncthreads();
+    for (int tile = t0; tile < t1; ++tile) {
+      take_bc();
+      if (tile + 1 < t1) load_bc(rows_of(tile + 1));
+      save();
+      if (rows_of(tile) > 0) scan((tile - t0) & 1);
+      __syncthreads();
+    }
+    end();
+  }
 }
 
 // One token of each sequence: four lanes to a channel, lane q of them the states
@@ -261,33 +295,38 @@ __global__ __launch_bounds__(256) void ssm_step_kernel(Ssm p, float* state) {
 template <typename T, int W, int NP, bool VEC>
 hipError_t fwd_launch(const Ssm& p, hipStream_t st) {
   const int nblk = p.G * p.gblocks;
+  const dim3 block(64 * (W + SSM_HELPERS));
   if (p.S > 1) {
     hipLaunchKernelGGL((ssm_fwd_kernel<T, W, NP, VEC, true>), dim3(nblk * (p.S - 1) * p.batch),
-                       dim3(64 * W), 0, st, p);
+                       block, 0, st, p);
     if (hipError_t e = hipGetLastError(); e != hipSuccess) return e;
   }
-  hipLaunchKernelGGL((ssm_fwd_kernel<T, W, NP, VEC, false>), dim3(nblk * p.S * p.batch),
-                     dim3(64 * W), 0, st, p);
+  hipLaunchKernelGGL((ssm_fwd_kernel<T, W, NP, VEC, false>), dim3(nblk * p.S * p.batch), block,
+                     0, st, p);
   return hipGetLastError();
 }
 
 template <typename T, bool VEC>
 hipError_t fwd_waves(const Ssm& p, hipStream_t st) {
-  switch (ssm_waves(p.N)) {
+  const SsmWaves n = ssm_fwd_waves(p.N);
+  switch (n.W) {
     case 1: return fwd_launch<T, 1, 1, VEC>(p, st);
     case 2: return fwd_launch<T, 2, 1, VEC>(p, st);
     case 4: return fwd_launch<T, 4, 1, VEC>(p, st);
-    default:
-      return ssm_passes(p.N) == 1 ? fwd_launch<T, 8, 1, VEC>(p, st) : fwd_launch<T, 8, 2, VEC>(p, st);
+    default: return n.NP == 1 ? fwd_launch<T, 8, 1, VEC>(p, st) : fwd_launch<T, 8, 2, VEC>(p, st);
   }
 }
 
-// Segments of a sequence: as many as bring the waves to two a SIMD
-int ssm_segments(int batch, int G, int Eg, int N, int L, bool) {
-  const int tiles = (L + SSM_TT - 1) / SSM_TT;
-  const long long waves = (long long)batch * G * ((Eg + SSM_CH - 1) / SSM_CH) * ssm_waves(N);
-  const long long want = 8LL * device_geom().cus;
-  long long s = want / waves;
+// Segments of a sequence.  One where the 64-channel blocks fill the chip, as a pass over
+// the segments' own states costs half the walk again (B = 4, E = 4096, N = 16: 256 blocks;
+// two segments took the training pass from 730 to 816 us).  Else as many as bring the
+// forward to three workgroups a CU (B = 1, L = 2048, E = 4096: 86, 79, 80 and 84 us at one
+// to four; L = 16384, E = 2048: 346, 273, 260, 265), the backward, whose LDS leaves room for
+// one, to one; of four tiles at least.
+int ssm_segments(int batch, int G, int Eg, int L, bool backward) {
+  const int tiles = (L + SSM_TT - 1) / SSM_TT, cus = device_geom().cus;
+  const long long groups = (long long)batch * G * ((Eg + SSM_CH - 1) / SSM_CH);
+  long long s = groups >= cus ? 1 : backward ? cus / groups : (3 * cus + groups - 1) / groups;
   if (s > tiles / 4) s = tiles / 4;
   if (s > 64) s = 64;
   if (s < 1) s = 1;

@@ -8,13 +8,18 @@
 namespace lz {
 
 // Layout of the work.  A workgroup takes 64 channels of one group and one sequence (or a
-// segment of it) and walks it in tiles of 16 tokens; a lane is a channel, and wave w of
-// its W holds the states n = 4 w .. 4 w + 3 (and 4 (w + W) .. with NP = 2), four a lane,
-// in registers.
+// segment of it) and walks it in tiles of 16 tokens.  In its W scan waves a lane is a
+// channel; wave w holds the states n = 4 w .. 4 w + 3 (and 4 (w + W) .. up to NP such),
+// four a lane, in registers.  Four helper waves turn the next tile's rows into delta, u and
+// the like while the scan waves walk this one, and the last tile's sums into rows: one
+// barrier a tile, and waves to switch between though a wave holds 256 states.  (With the
+// scan waves doing both, two barriers a tile, the training pass of 8192 tokens x 4096
+// channels x 16 states took 857 us where this takes 738.)
+// In LDS a tile is rows of the 64 channels: a thread's share of a row is one vector, a
+// wave's read of a token 64 consecutive floats (channels of 16 tokens each, 20 floats
+// apart, made the transposed writes and reads conflict: 40 % of the forward's time).
 constexpr int SSM_CH = 64, SSM_TT = 16, SSM_MAX_STATE = 64;
-constexpr int SSM_PITCH = SSM_TT + 4;   // floats from one channel to the next in LDS: 16-byte
-                                        // reads of 16 lanes fall on all 64 banks
-constexpr int SSM_TILE = SSM_CH * SSM_PITCH;
+constexpr int SSM_TILE = SSM_CH * SSM_TT;
 
 struct Ssm {
   const void *x, *dt, *z, *B, *C;
@@ -42,16 +47,17 @@ struct SsmGrad {
   float* part_d;         // [B S, 2, E]: of dD and ddt_bias
   float* rec;            // as Ssm's, of the reverse walk
   float* dsum;
+  float* acc;            // [3][B, L, E]: sums over the states of earlier launches
+  long long acc_step;    // B L E
+  int n0, first, last;   // this launch's first state; whether it is the first, the last
+  int NQ;                // padded states in part_bc
 };
 
-// The V elements a thread takes of R rows of a tile, W waves to a workgroup
-template <int W>
-struct SsmSplit {
-  static constexpr int V = 16 / W < 8 ? 16 / W : 8;
-  static constexpr int R = 16 / (W * V);
-  static constexpr int COLS = SSM_CH / V;          // threads to a row
-  static constexpr int ROWS = 64 * W / COLS;       // rows at a time
-};
+// Helper waves of a workgroup, and what a thread of theirs takes of a tile: V channels of
+// one row
+constexpr int SSM_HELPERS = 4, SSM_V = SSM_TILE / (64 * SSM_HELPERS);
+constexpr int SSM_COLS = SSM_CH / SSM_V, SSM_ROWS = 64 * SSM_HELPERS / SSM_COLS;
+static_assert(SSM_V == 4 && SSM_ROWS == SSM_TT, "a thread, a vector of the tile");
 
 template <class F, int... K>
 __device__ __forceinline__ void static_for_impl(F f, std::integer_sequence<int, K...>) {
@@ -60,6 +66,26 @@ __device__ __forceinline__ void static_for_impl(F f, std::integer_sequence<int, 
 template <int N, class F>
 __device__ __forceinline__ void static_for(F f) {
   static_for_impl(f, std::make_integer_sequence<int, N>{});
+}
+
+// A thread's vector of a tile
+__device__ __forceinline__ void put_row(float* to, const float (&v)[SSM_V]) {
+  *reinterpret_cast<f32x4*>(to) = f32x4{v[0], v[1], v[2], v[3]};
+}
+__device__ __forceinline__ void add_row(float (&v)[SSM_V], const float* from) {
+  const f32x4 x = *reinterpret_cast<const f32x4*>(from);
+#pragma unroll
+  for (int k = 0; k < SSM_V; ++k) v[k] += x[k];
+}
+// Four tokens of a lane's channel
+__device__ __forceinline__ f32x4 get_tokens(const float* tile, int t, int lane) {
+  const float* p = tile + t * SSM_CH + lane;
+  return f32x4{p[0], p[SSM_CH], p[2 * SSM_CH], p[3 * SSM_CH]};
+}
+__device__ __forceinline__ void put_tokens(float* tile, int t, int lane, const f32x4& v) {
+  float* p = tile + t * SSM_CH + lane;
+#pragma unroll
+  for (int k = 0; k < 4; ++k) p[k * SSM_CH] = v[k];
 }
 
 // B or C of a tile for the four states of a wave: register i of a lane holds token
@@ -104,6 +130,20 @@ __device__ __forceinline__ void ssm_dots(f32x4& y, float v, const float (&h)[4][
   y = f32x4{y0, y1, y2, y3};
 }
 
+// g[n] = v(K + n) x + c[n], likewise
+template <int K>
+__device__ __forceinline__ void ssm_fma4(float (&g)[4], float v, float x, const float (&c)[4]) {
+  float g0 = c[0], g1 = c[1], g2 = c[2], g3 = c[3];
+  asm("s_nop 1\n"
+      "v_fmac_f32_dpp %0, %4, %5 row_newbcast:%6 row_mask:0xf bank_mask:0xf\n"
+      "v_fmac_f32_dpp %1, %4, %5 row_newbcast:%7 row_mask:0xf bank_mask:0xf\n"
+      "v_fmac_f32_dpp %2, %4, %5 row_newbcast:%8 row_mask:0xf bank_mask:0xf\n"
+      "v_fmac_f32_dpp %3, %4, %5 row_newbcast:%9 row_mask:0xf bank_mask:0xf\n"
+      : "+&v"(g0), "+&v"(g1), "+&v"(g2), "+&v"(g3)
+      : "v"(v), "v"(x), "n"(K), "n"(K + 1), "n"(K + 2), "n"(K + 3));
+  g[0] = g0, g[1] = g1, g[2] = g2, g[3] = g3;
+}
+
 // Where a workgroup works
 struct SsmPlace {
   int b, s, blk, g, c0, cols;   // sequence, segment, block; group, first channel, channels
@@ -125,10 +165,19 @@ struct SsmPlace {
   }
 };
 
-inline int ssm_waves(int N) { return N <= 4 ? 1 : N <= 8 ? 2 : N <= 16 ? 4 : 8; }
-inline int ssm_passes(int N) { return N <= 32 ? 1 : 2; }
+// Scan waves W and passes NP of the forward for N states
+struct SsmWaves {
+  int W, NP;
+};
+inline SsmWaves ssm_fwd_waves(int N) {
+  return N <= 4 ? SsmWaves{1, 1} : N <= 8 ? SsmWaves{2, 1} : N <= 16 ? SsmWaves{4, 1}
+       : N <= 32 ? SsmWaves{8, 1} : SsmWaves{8, 2};
+}
+// States the backward takes a launch, and N in whole waves
+constexpr int SSM_BWD_STATES = 16;
+inline int ssm_bwd_padded(int N) { return (N + 3) / 4 * 4 <= 4 ? 4 : N <= 8 ? 8 : (N + 15) / 16 * 16; }
 
-int ssm_segments(int batch, int G, int Eg, int N, int L, bool backward);
+int ssm_segments(int batch, int G, int Eg, int L, bool backward);
 hipError_t launch_ssm_fwd(const Ssm& p, bool is_bf16, bool vec, hipStream_t st);
 hipError_t launch_ssm_step(const Ssm& p, float* state, bool is_bf16, hipStream_t st);
 hipError_t launch_ssm_bwd(const Ssm& p, const SsmGrad& g, void* dB, void* dC, float* dA,

@@ -14,7 +14,8 @@
 // is added across the wave, eight sums at a time, each step halving the lanes that carry
 // one (17 instructions for the 8 sums of 64 lanes), and its 64-channel shares, as the
 // sequences' shares of dA, dD and dbias, go to memory for a second launch that adds them in
-// order: no atomics, the same bits every time.
+// order: no atomics, the same bits every time.  More than 16 states are taken 16 a launch
+// (in one, a wave's registers did not hold them: N = 24 took 2.8 times as long as 16).
 #include "ssm.hpp"
 
 namespace lz {
@@ -54,19 +55,24 @@ __device__ __forceinline__ float wave_sums8(const float (&v)[8]) {
   return s;
 }
 
-// The walk of both backward kernels over a segment: with STATE only the carried gradient,
-// to rec, and the sum of delta, for the segments but the first.
-template <typename T, int W, int NP, bool VEC, bool STATE>
-__global__ __launch_bounds__(64 * W, W == 8 ? 2 : W == 4 ? 2 : 1) void ssm_bwd_kernel(Ssm p, SsmGrad gr) {
-  using Split = SsmSplit<W>;
-  constexpr int V = Split::V, R = Split::R;
+// STATE: the gradient that a segment carries back alone, and its sum of delta, for the
+// segments but the first.
+template <int W, bool STATE>
+constexpr int ssm_bwd_lds() {   // tiles, two of each
+  return 2 * (STATE ? 2 : 3 + 3 * W);
+}
+
+template <typename T, int W, bool VEC, bool STATE>
+__global__ __launch_bounds__(64 * (W + SSM_HELPERS), 2) void ssm_bwd_kernel(Ssm p, SsmGrad gr) {
+  constexpr int V = SSM_V;
   extern __shared__ float lds[];
-  float* const sd = lds;                    // delta
-  float* const su = sd + SSM_TILE;          // delta x
-  float* const sg = su + SSM_TILE;          // dm
-  float* const pu = sg + SSM_TILE;          // [W]: the waves' shares of du,
-  float* const pd = pu + W * SSM_TILE;      // of sum_n v A
-  float* const py = pd + W * SSM_TILE;      // and of sum_n C h
+  auto sd = [&](int buf) { return lds + buf * SSM_TILE; };              // delta
+  auto sg = [&](int buf) { return lds + (2 + buf) * SSM_TILE; };      // dm
+  auto su = [&](int buf) { return lds + (4 + buf) * SSM_TILE; };  // delta x
+  // the waves' shares of du, of sum_n v A and of sum_n C h
+  auto pu = [&](int buf, int j) { return lds + ((3 + j) * 2 + buf) * SSM_TILE; };
+  auto pd = [&](int buf, int j) { return lds + ((3 + W + j) * 2 + buf) * SSM_TILE; };
+  auto py = [&](int buf, int j) { return lds + ((3 + 2 * W + j) * 2 + buf) * SSM_TILE; };
   const int segments = STATE ? p.S - 1 : p.S;
   SsmPlace at(p, segments);
   if constexpr (STATE) {   // segments 1 .. S - 1
@@ -74,326 +80,360 @@ __global__ __launch_bounds__(64 * W, W == 8 ? 2 : W == 4 ? 2 : 1) void ssm_bwd_k
     at.tile0 = at.s * p.seg_tiles;
     at.tile1 = min(p.tiles, at.tile0 + p.seg_tiles);
   }
-  const int tid = threadIdx.x, lane = tid & 63;
-  const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int c = at.c0 + lane;
-  const bool mine = lane < at.cols;
-  const int N = p.N, E = p.E;
-
-  float A2[NP][4], carry[NP][4], dA[NP][4];
-#pragma unroll
-  for (int q = 0; q < NP; ++q)
-#pragma unroll
-    for (int k = 0; k < 4; ++k) {
-      const int n = 4 * (w + W * q) + k;
-      A2[q][k] = mine && n < N ? p.A[(size_t)c * N + n] * LOG2E : 0.f;
-      carry[q][k] = dA[q][k] = 0.f;
-    }
-  if constexpr (!STATE) {
-    // what the later segments carry back
-    for (int j = p.S - 1; j > at.s; --j) {
-      const size_t rec = (size_t)at.b * (p.S - 1) + j - 1;
-      const float d = mine ? gr.dsum[rec * E + c] : 0.f;
-#pragma unroll
-      for (int q = 0; q < NP; ++q)
-#pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          const int n = 4 * (w + W * q) + k;
-          if (mine && n < N)
-            carry[q][k] = fmaf(__builtin_amdgcn_exp2f(A2[q][k] * d), carry[q][k],
-                               gr.rec[(rec * N + n) * E + c]);
-        }
-    }
-  }
-
-  const int tr = tid / Split::COLS, tc = (tid % Split::COLS) * V, left = at.cols - tc;
-  float bias[V], D[V], dD[V], dbias[V];
-#pragma unroll
-  for (int i = 0; i < V; ++i) {
-    bias[i] = p.bias && i < left ? p.bias[at.c0 + tc + i] : 0.f;
-    D[i] = p.D && i < left ? p.D[at.c0 + tc + i] : 0.f;
-    dD[i] = dbias[i] = 0.f;
-  }
-  const long long last = (long long)(at.tile1 - 1) * SSM_TT;
-  const int x_t = p.x_t, dt_t = p.dt_t, z_t = p.z_t, B_t = p.B_t, C_t = p.C_t;
+  const int lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int E = p.E, N = p.N;
   const bool has_z = p.z, soft = p.softplus;
+  const long long last = (long long)(at.tile1 - 1) * SSM_TT;
+  auto rows_of = [&](int tile) { return min(SSM_TT, p.L - tile * SSM_TT); };
+
+  // --- rows to delta, u and dm; the waves' shares to gradients (helper) ------------------
+  const int tid = (int)threadIdx.x - 64 * W;
+  const int row = tid / SSM_COLS, tc = (tid % SSM_COLS) * V, left = at.cols - tc;
+  float bias[V], D[V], dD[V], dbias[V];
+  const int x_t = p.x_t, dt_t = p.dt_t, z_t = p.z_t;
   const T* xb = (const T*)p.x + at.b * p.x_b + last * x_t + at.c0;
   const T* db = (const T*)p.dt + at.b * p.dt_b + last * dt_t + at.c0;
   const T* zb = has_z ? (const T*)p.z + at.b * p.z_b + last * z_t + at.c0 : nullptr;
-  const T* Bb = (const T*)p.B + at.b * p.B_b + last * B_t + (long long)at.g * p.B_g;
-  const T* Cb = (const T*)p.C + at.b * p.C_b + last * C_t + (long long)at.g * p.C_g;
-  long long yo = ((long long)at.b * p.L + last) * E + at.c0;   // rows of dy, next to load
-  const T* dyb = (const T*)gr.dy + yo;
-  const float* saved = p.saved + ((size_t)at.b * p.tiles + at.tile1 - 1) * N * E + c;
-  const int NQ = 4 * W * NP;
-  float* bc = STATE ? nullptr
-                    : gr.part_bc + (((long long)at.blk * p.batch + at.b) * p.L + last) * 2 * NQ;
-
-  RawRow<T, V, VEC> xr[R], dr[R], zr[R], yr[R];
-  SsmVec<T> Bv[NP], Cv[NP];
-  float h0[NP][4];
-  auto load = [&](int rows) {
-    const rsrc_t rx = open_rsrc(xb), rd = open_rsrc(db), rz = open_rsrc(zb), ry = open_rsrc(dyb);
+  const T* dyb = (const T*)gr.dy + ((long long)at.b * p.L + last) * E + at.c0;
+  struct Rows {
+    RawRow<T, V, VEC> x, dt, z, dy;
+  } next;
+  auto load_params = [&] {
 #pragma unroll
-    for (int r = 0; r < R; ++r) {
-      const int row = tr + r * Split::ROWS;
-      xr[r] = load_raw<T, V, VEC>(rx, row * x_t + tc, row < rows, left);
-      dr[r] = load_raw<T, V, VEC>(rd, row * dt_t + tc, row < rows, left);
-      zr[r] = load_raw<T, V, VEC>(rz, row * z_t + tc, has_z && row < rows, left);
-      yr[r] = load_raw<T, V, VEC>(ry, row * E + tc, row < rows, left);
+    for (int i = 0; i < V; ++i) {
+      bias[i] = p.bias && i < left ? p.bias[at.c0 + tc + i] : 0.f;
+      D[i] = p.D && i < left ? p.D[at.c0 + tc + i] : 0.f;
+      dD[i] = dbias[i] = 0.f;
     }
-#pragma unroll
-    for (int q = 0; q < NP; ++q) {
-      if (!STATE) Bv[q].load(Bb, rows, B_t, N, 4 * (w + W * q), lane);
-      Cv[q].load(Cb, rows, C_t, N, 4 * (w + W * q), lane);
-      if (!STATE) {
-#pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          const int n = 4 * (w + W * q) + k;
-          h0[q][k] = mine && n < N ? saved[(size_t)n * E] : 0.f;
-        }
-      }
+  };
+  auto load_rows = [&](int rows) {
+    const rsrc_t rx = open_rsrc(xb), rd = open_rsrc(db), rz = open_rsrc(zb), ry = open_rsrc(dyb);
+    {
+      if (!STATE) next.x = load_raw<T, V, VEC>(rx, row * x_t + tc, row < rows, left);
+      next.dt = load_raw<T, V, VEC>(rd, row * dt_t + tc, row < rows, left);
+      next.z = load_raw<T, V, VEC>(rz, row * z_t + tc, has_z && row < rows, left);
+      next.dy = load_raw<T, V, VEC>(ry, row * E + tc, row < rows, left);
     }
     xb -= SSM_TT * (long long)x_t;
     db -= SSM_TT * (long long)dt_t;
     if (has_z) zb -= SSM_TT * (long long)z_t;
     dyb -= SSM_TT * (long long)E;
+  };
+  auto prep = [&](int rows, int buf) {
+    {
+      const int e = row * SSM_CH + tc;
+      float d[V], u[V], dm[V];
+#pragma unroll
+      for (int i = 0; i < V; ++i) {
+        const float pre = next.dt.at(i) + bias[i], z = next.z.at(i), dy = next.dy.at(i);
+        d[i] = row < rows ? soft ? softplus(pre) : pre : 0.f;
+        dm[i] = has_z ? dy * (z * sigmoid(z)) : dy;
+        if (!STATE) u[i] = d[i] * next.x.at(i);
+      }
+      put_row(sd(buf) + e, d);
+      put_row(sg(buf) + e, dm);
+      if (!STATE) put_row(su(buf) + e, u);
+    }
+  };
+  auto finish = [&](int tile, int buf, const Rows& now) {
+    const int rows = rows_of(tile), e = row * SSM_CH + tc;
+    const long long o = ((long long)at.b * p.L + (long long)tile * SSM_TT) * E + at.c0;
+    const uint32_t off = row * E + tc;
+    const bool in = row < rows;
+    float sum[3][V];   // of du, of sum_n v A and of sum_n C h
+#pragma unroll
+    for (int i = 0; i < V; ++i) sum[0][i] = sum[1][i] = 0.f, sum[2][i] = now.x.at(i) * D[i];
+    if (!gr.first) {
+#pragma unroll
+      for (int k = 0; k < 3; ++k) {
+        const auto r = load_raw<float, V, VEC>(open_rsrc(gr.acc + k * gr.acc_step + o), off, in, left);
+#pragma unroll
+        for (int i = 0; i < V; ++i) sum[k][i] = r.at(i);
+      }
+    }
+#pragma unroll
+    for (int j = 0; j < W; ++j) {
+      add_row(sum[0], pu(buf, j) + e);
+      add_row(sum[1], pd(buf, j) + e);
+      if (has_z) add_row(sum[2], py(buf, j) + e);
+    }
+    if (!gr.last) {
+#pragma unroll
+      for (int k = 0; k < 3; ++k) {
+        RawRow<float, V, VEC> r;
+#pragma unroll
+        for (int i = 0; i < V; ++i) r.set(i, sum[k][i]);
+        store_raw<float, V, VEC>(open_rsrc(gr.acc + k * gr.acc_step + o), off, in, left, r);
+      }
+      return;
+    }
+    RawRow<T, V, VEC> ox, od, oz;
+    float d[V] = {0.f, 0.f, 0.f, 0.f};
+    add_row(d, sd(buf) + e);
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+      const float x = now.x.at(i), dy = now.dy.at(i);
+      float dm = dy, ddt = fmaf(x, sum[0][i], sum[1][i] * LN2);
+      if (has_z) {
+        const float z = now.z.at(i), sz = sigmoid(z);
+        dm = dy * (z * sz);
+        oz.set(i, dy * sum[2][i] * (sz * fmaf(z, 1.f - sz, 1.f)));
+      }
+      if (soft) ddt *= sigmoid(now.dt.at(i) + bias[i]);
+      ox.set(i, fmaf(d[i], sum[0][i], D[i] * dm));
+      od.set(i, ddt);
+      if (in && i < left) {
+        dD[i] += dm * x;
+        dbias[i] += ddt;
+      }
+    }
+    store_raw<T, V, VEC>(open_rsrc((T*)gr.dx + o), off, in, left, ox);
+    store_raw<T, V, VEC>(open_rsrc((T*)gr.ddt + o), off, in, left, od);
+    if (has_z) store_raw<T, V, VEC>(open_rsrc((T*)gr.dz + o), off, in, left, oz);
+  };
+
+  // --- the walk (scan) --------------------------------------------------------------------
+  const int w = wave, c = at.c0 + lane, n0 = gr.n0 + 4 * w;
+  const bool mine = lane < at.cols;
+  const int B_t = p.B_t, C_t = p.C_t;
+  const T* Bb = (const T*)p.B + at.b * p.B_b + last * B_t + (long long)at.g * p.B_g;
+  const T* Cb = (const T*)p.C + at.b * p.C_b + last * C_t + (long long)at.g * p.C_g;
+  const float* saved = p.saved + ((size_t)at.b * p.tiles + at.tile1 - 1) * N * E + c;
+  float* bc = STATE ? nullptr
+                    : gr.part_bc + (((long long)at.blk * p.batch + at.b) * p.L + last) * 2 * gr.NQ;
+  const int NQ = gr.NQ;
+  float A2[4], carry[4], dA[4], dsum = 0.f;
+  SsmVec<T> Bv, Cv;
+  float h0[4];
+  auto start = [&] {
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const int n = n0 + k;
+        A2[k] = mine && n < N ? p.A[(size_t)c * N + n] * LOG2E : 0.f;
+        carry[k] = dA[k] = 0.f;
+      }
+    if constexpr (!STATE) {
+      // what the later segments carry back
+      for (int j = p.S - 1; j > at.s; --j) {
+        const size_t rec = (size_t)at.b * (p.S - 1) + j - 1;
+        const float d = mine ? gr.dsum[rec * E + c] : 0.f;
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            const int n = n0 + k;
+            if (mine && n < N)
+              carry[k] = fmaf(__builtin_amdgcn_exp2f(A2[k] * d), carry[k],
+                                 gr.rec[(rec * N + n) * E + c]);
+          }
+      }
+    }
+  };
+  auto load_bc = [&](int rows) {
+    if (!STATE) Bv.load(Bb, rows, B_t, N, n0, lane);
+    Cv.load(Cb, rows, C_t, N, n0, lane);
+    if (!STATE) {
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const int n = n0 + k;
+        h0[k] = mine && n < N ? saved[(size_t)n * E] : 0.f;
+      }
+    }
+  };
+  auto next_bc = [&] {
     Bb -= SSM_TT * (long long)B_t;
     Cb -= SSM_TT * (long long)C_t;
     saved -= (size_t)N * E;
   };
-
-  float dsum = 0.f;
-  load(min(SSM_TT, p.L - (int)last));
-  for (int tile = at.tile1 - 1; tile >= at.tile0; --tile) {
-    const int t0 = tile * SSM_TT;
-    const int rows = min(SSM_TT, p.L - t0);
-    float xv[R][V], dl[R][V], sl[R][V], zv[R][V], dyv[R][V];
+  auto scan_state = [&](int buf) {
+    float Cf[4];
 #pragma unroll
-    for (int r = 0; r < R; ++r) {
-      const int row = tr + r * Split::ROWS;
+    for (int i = 0; i < 4; ++i) Cf[i] = Cv.at(i);
 #pragma unroll
-      for (int i = 0; i < V; ++i) {
-        const float x = xr[r].at(i), pre = dr[r].at(i) + bias[i], z = zr[r].at(i);
-        const float dy = yr[r].at(i);
-        const float d = row < rows ? soft ? softplus(pre) : pre : 0.f;
-        const float dm = has_z ? dy * (z * sigmoid(z)) : dy;
-        sd[(tc + i) * SSM_PITCH + row] = d;
-        sg[(tc + i) * SSM_PITCH + row] = dm;
-        if (!STATE) su[(tc + i) * SSM_PITCH + row] = d * x;
-        xv[r][i] = x, dl[r][i] = d, sl[r][i] = soft ? sigmoid(pre) : 1.f;
-        zv[r][i] = z, dyv[r][i] = dy;
-      }
+    for (int i = 3; i >= 0; --i) {
+      const f32x4 d4 = get_tokens(sd(buf), 4 * i, lane), g4 = get_tokens(sg(buf), 4 * i, lane);
+      dsum += (d4[0] + d4[1]) + (d4[2] + d4[3]);
+      static_for<4>([&](auto kt) {
+        constexpr int t = 3 - decltype(kt)::value;
+        float g[4];
+        ssm_fma4<4 * t>(g, Cf[i], g4[t], carry);
+#pragma unroll
+        for (int n = 0; n < 4; ++n) carry[n] = __builtin_amdgcn_exp2f(d4[t] * A2[n]) * g[n];
+      });
     }
-    float Bf[NP][4], Cf[NP][4], hb[NP][4];
+  };
+  auto scan = [&](int tile, int buf, bool more) {
+    const int rows = rows_of(tile);
+    float a[16][4], h[16][4], Bf[4], Cf[4], hb[4], bcsum[2] = {0.f, 0.f};
 #pragma unroll
-    for (int q = 0; q < NP; ++q)
+    for (int i = 0; i < 4; ++i) Bf[i] = Bv.at(i), Cf[i] = Cv.at(i), hb[i] = h0[i];
+    if (more) load_bc(SSM_TT);
+    // forward over the tile
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        if (!STATE) Bf[q][i] = Bv[q].at(i);
-        Cf[q][i] = Cv[q].at(i);
-        if (!STATE) hb[q][i] = h0[q][i];
-      }
-    if (tile > at.tile0) load(SSM_TT);
-    __syncthreads();
-    if constexpr (STATE) {
-#pragma unroll
-      for (int i = 3; i >= 0; --i) {
-        const f32x4 d4 = *reinterpret_cast<const f32x4*>(sd + lane * SSM_PITCH + 4 * i);
-        const f32x4 g4 = *reinterpret_cast<const f32x4*>(sg + lane * SSM_PITCH + 4 * i);
-        dsum += (d4[0] + d4[1]) + (d4[2] + d4[3]);
-        static_for<4>([&](auto kt) {
-          constexpr int t = 3 - decltype(kt)::value;
-#pragma unroll
-          for (int q = 0; q < NP; ++q)
-            static_for<4>([&](auto kn) {
-              constexpr int n = decltype(kn)::value;
-              carry[q][n] = __builtin_amdgcn_exp2f(d4[t] * A2[q][n]) *
-                            (dpp<DPP_BCAST + 4 * t + n>(Cf[q][i]) * g4[t] + carry[q][n]);
-            });
+    for (int i = 0; i < 4; ++i) {
+      const f32x4 d4 = get_tokens(sd(buf), 4 * i, lane), u4 = get_tokens(su(buf), 4 * i, lane);
+      float hs[4][4];
+      static_for<4>([&](auto kt) {
+        constexpr int t = decltype(kt)::value;
+        static_for<4>([&](auto kn) {
+          constexpr int n = decltype(kn)::value;
+          const float before = 4 * i + t ? h[(4 * i + t + 15) % 16][n] : hb[n];
+          a[4 * i + t][n] = __builtin_amdgcn_exp2f(d4[t] * A2[n]);
+          h[4 * i + t][n] = fmaf(a[4 * i + t][n], before,
+                                 dpp<DPP_BCAST + 4 * t + n>(Bf[i]) * u4[t]);
+          hs[t][n] = h[4 * i + t][n];
         });
-      }
-    } else {
-      float bcsum[NP][2];
-#pragma unroll
-      for (int q = 0; q < NP; ++q) {
-        float a[16][4], h[16][4];
-        // forward over the tile
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const f32x4 d4 = *reinterpret_cast<const f32x4*>(sd + lane * SSM_PITCH + 4 * i);
-          const f32x4 u4 = *reinterpret_cast<const f32x4*>(su + lane * SSM_PITCH + 4 * i);
-          float hs[4][4];
-          static_for<4>([&](auto kt) {
-            constexpr int t = decltype(kt)::value;
-            static_for<4>([&](auto kn) {
-              constexpr int n = decltype(kn)::value;
-              const float before = 4 * i + t ? h[(4 * i + t + 15) % 16][n] : hb[q][n];
-              a[4 * i + t][n] = __builtin_amdgcn_exp2f(d4[t] * A2[q][n]);
-              h[4 * i + t][n] = fmaf(a[4 * i + t][n], before,
-                                     dpp<DPP_BCAST + 4 * t + n>(Bf[q][i]) * u4[t]);
-              hs[t][n] = h[4 * i + t][n];
-            });
-          });
-          if (has_z) {
-            float* to = py + w * SSM_TILE + lane * SSM_PITCH + 4 * i;
-            f32x4 yl = {0.f, 0.f, 0.f, 0.f};
-            if (q) yl = *reinterpret_cast<const f32x4*>(to);
-            ssm_dots(yl, Cf[q][i], hs);
-            *reinterpret_cast<f32x4*>(to) = yl;
-          }
-        }
-        // and back
-        bcsum[q][0] = bcsum[q][1] = 0.f;
-#pragma unroll
-        for (int i = 3; i >= 0; --i) {
-          const f32x4 d4 = *reinterpret_cast<const f32x4*>(sd + lane * SSM_PITCH + 4 * i);
-          const f32x4 u4 = *reinterpret_cast<const f32x4*>(su + lane * SSM_PITCH + 4 * i);
-          const f32x4 g4 = *reinterpret_cast<const f32x4*>(sg + lane * SSM_PITCH + 4 * i);
-          float gs[4][4];
-          f32x4 dv = {0.f, 0.f, 0.f, 0.f}, du = {0.f, 0.f, 0.f, 0.f};
-          float* const tu = pu + w * SSM_TILE + lane * SSM_PITCH + 4 * i;
-          float* const td = pd + w * SSM_TILE + lane * SSM_PITCH + 4 * i;
-          if (q) {
-            dv = *reinterpret_cast<const f32x4*>(td);
-            du = *reinterpret_cast<const f32x4*>(tu);
-          }
-          static_for<4>([&](auto kt) {
-            constexpr int t = 3 - decltype(kt)::value;
-            const int tt = 4 * i + t;
-            float v8[8];
-            static_for<4>([&](auto kn) {
-              constexpr int n = decltype(kn)::value;
-              const float g = dpp<DPP_BCAST + 4 * t + n>(Cf[q][i]) * g4[t] + carry[q][n];
-              gs[t][n] = g;
-              v8[n] = g * u4[t];
-              v8[4 + n] = g4[t] * h[tt][n];
-              carry[q][n] = a[tt][n] * g;
-              const float v = carry[q][n] * (tt ? h[(tt + 15) % 16][n] : hb[q][n]);
-              dv[t] = fmaf(v, A2[q][n], dv[t]);
-              dA[q][n] = fmaf(v, d4[t], dA[q][n]);
-            });
-            const float s8 = wave_sums8(v8);
-            if ((lane & 7) == (tt & 7)) bcsum[q][tt >> 3] = s8;
-          });
-          ssm_dots(du, Bf[q][i], gs);
-          *reinterpret_cast<f32x4*>(td) = dv;
-          *reinterpret_cast<f32x4*>(tu) = du;
-        }
-        // lane l: of token l % 8 (+ 8), B's (l < 32) or C's sum for state (l / 8) % 4
-        const rsrc_t rb = open_rsrc(bc);
-#pragma unroll
-        for (int k = 0; k < 2; ++k) {
-          const int row = 8 * k + (lane & 7), idx = lane >> 3;
-          const uint32_t off =
-              (uint32_t)((2 * row + (idx >> 2)) * NQ + 4 * (w + W * q) + (idx & 3)) * 4u;
-          __builtin_amdgcn_raw_buffer_store_b32(__builtin_bit_cast(uint32_t, bcsum[q][k]), rb,
-                                                row < rows ? off : OOB, 0, 0);
-        }
-      }
-      bc -= SSM_TT * 2 * NQ;
-    }
-    __syncthreads();
-    if constexpr (!STATE) {
-      const long long o = ((long long)at.b * p.L + t0) * E + at.c0;
-      const rsrc_t rx = open_rsrc((T*)gr.dx + o), rd = open_rsrc((T*)gr.ddt + o);
-      const rsrc_t rz = open_rsrc(has_z ? (T*)gr.dz + o : nullptr);
-#pragma unroll
-      for (int r = 0; r < R; ++r) {
-        const int row = tr + r * Split::ROWS;
-        RawRow<T, V, VEC> ox, od, oz;
-#pragma unroll
-        for (int i = 0; i < V; ++i) {
-          const int e = (tc + i) * SSM_PITCH + row;
-          float du = 0.f, dv = 0.f, y = xv[r][i] * D[i];
-#pragma unroll
-          for (int j = 0; j < W; ++j) {
-            du += pu[j * SSM_TILE + e];
-            dv += pd[j * SSM_TILE + e];
-            if (has_z) y += py[j * SSM_TILE + e];
-          }
-          const float z = zv[r][i], sz = sigmoid(z), dy = dyv[r][i];
-          const float dm = has_z ? dy * (z * sz) : dy;
-          const float ddt = fmaf(xv[r][i], du, dv * LN2) * sl[r][i];
-          ox.set(i, fmaf(dl[r][i], du, D[i] * dm));
-          od.set(i, ddt);
-          if (has_z) oz.set(i, dy * y * (sz * (1.f + z * (1.f - sz))));
-          if (row < rows && i < left) {
-            dD[i] += dm * xv[r][i];
-            dbias[i] += ddt;
-          }
-        }
-        store_raw<T, V, VEC>(rx, row * E + tc, row < rows, left, ox);
-        store_raw<T, V, VEC>(rd, row * E + tc, row < rows, left, od);
-        if (has_z) store_raw<T, V, VEC>(rz, row * E + tc, row < rows, left, oz);
+      });
+      if (has_z) {
+        f32x4 yl = {0.f, 0.f, 0.f, 0.f};
+        ssm_dots(yl, Cf[i], hs);
+        put_tokens(py(buf, w), 4 * i, lane, yl);
       }
     }
-  }
-
-  if constexpr (STATE) {
+    // and back
+#pragma unroll
+    for (int i = 3; i >= 0; --i) {
+      const f32x4 d4 = get_tokens(sd(buf), 4 * i, lane), u4 = get_tokens(su(buf), 4 * i, lane);
+      const f32x4 g4 = get_tokens(sg(buf), 4 * i, lane);
+      float gs[4][4];
+      f32x4 dv = {0.f, 0.f, 0.f, 0.f}, du = {0.f, 0.f, 0.f, 0.f};
+      static_for<4>([&](auto kt) {
+        constexpr int t = 3 - decltype(kt)::value;
+        const int tt = 4 * i + t;
+        float v8[8];
+        ssm_fma4<4 * t>(gs[t], Cf[i], g4[t], carry);
+        static_for<4>([&](auto kn) {
+          constexpr int n = decltype(kn)::value;
+          const float g = gs[t][n];
+          v8[n] = g * u4[t];
+          v8[4 + n] = g4[t] * h[tt][n];
+          carry[n] = a[tt][n] * g;
+          const float v = carry[n] * (tt ? h[(tt + 15) % 16][n] : hb[n]);
+          dv[t] = fmaf(v, A2[n], dv[t]);
+          dA[n] = fmaf(v, d4[t], dA[n]);
+        });
+        const float s8 = wave_sums8(v8);
+        if ((lane & 7) == (tt & 7)) bcsum[tt >> 3] = s8;
+      });
+      ssm_dots(du, Bf[i], gs);
+      put_tokens(pd(buf, w), 4 * i, lane, dv);
+      put_tokens(pu(buf, w), 4 * i, lane, du);
+    }
+    // lane l: of token l % 8 (+ 8), B's (l < 32) or C's sum for state (l / 8) % 4
+    const rsrc_t rb = open_rsrc(bc);
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+      const int row = 8 * k + (lane & 7), idx = lane >> 3;
+      const uint32_t off =
+          (uint32_t)((2 * row + (idx >> 2)) * NQ + n0 + (idx & 3)) * 4u;
+      __builtin_amdgcn_raw_buffer_store_b32(__builtin_bit_cast(uint32_t, bcsum[k]), rb,
+                                            row < rows ? off : OOB, 0, 0);
+    }
+    bc -= SSM_TT * 2 * NQ;
+  };
+  auto end = [&] {
     if (!mine) return;
-    const size_t rec = (size_t)at.b * (p.S - 1) + at.s - 1;
-    if (w == 0) gr.dsum[rec * E + c] = dsum;
+    const size_t rec = (size_t)at.b * (p.S - 1) + at.s - 1, part = (size_t)at.b * p.S + at.s;
+    if (STATE && w == 0) gr.dsum[rec * E + c] = dsum;
 #pragma unroll
-    for (int q = 0; q < NP; ++q)
-#pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        const int n = 4 * (w + W * q) + k;
-        if (n < N) gr.rec[(rec * N + n) * E + c] = carry[q][k];
+    for (int k = 0; k < 4; ++k) {
+      const int n = n0 + k;
+      if (n >= N) continue;
+      if (STATE) gr.rec[(rec * N + n) * E + c] = carry[k];
+      else gr.part_a[(part * N + n) * E + c] = dA[k];
+    }
+  };
+
+  const int t0 = at.tile0, t1 = at.tile1;   // t0 < t1
+  if (wave >= W) {
+    Rows now, before;   // of this tile and the one after it in the sequence
+    load_params();
+    load_rows(rows_of(t1 - 1));
+    prep(rows_of(t1 - 1), 0);
+    now = next;
+    if (t1 - 1 > t0) load_rows(SSM_TT);
+    __syncthreads();
+    for (int tile = t1 - 1; tile >= t0; --tile) {
+      const int buf = (t1 - 1 - tile) & 1;
+      if (!STATE && tile < t1 - 1) finish(tile + 1, buf ^ 1, before);
+      before = now;
+      if (tile > t0) {
+        prep(SSM_TT, buf ^ 1);
+        now = next;
+        if (tile - 1 > t0) load_rows(SSM_TT);
       }
+      __syncthreads();
+    }
+    if (!STATE) finish(t0, (t1 - 1 - t0) & 1, before);
   } else {
-    const size_t part = (size_t)at.b * p.S + at.s;
-#pragma unroll
-    for (int q = 0; q < NP; ++q)
-#pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        const int n = 4 * (w + W * q) + k;
-        if (mine && n < N) gr.part_a[(part * N + n) * E + c] = dA[q][k];
+    load_bc(rows_of(t1 - 1));
+    next_bc();
+    start();
+    __syncthreads();
+    for (int tile = t1 - 1; tile >= t0; --tile) {
+      const int buf = (t1 - 1 - tile) & 1;
+      if constexpr (STATE) {
+        scan_state(buf);
+        if (tile > t0) load_bc(SSM_TT);
+      } else {
+        scan(tile, buf, tile > t0);
       }
-    // the rows' shares of dD and dbias meet in LDS (the delta and u tiles)
+      next_bc();
+      __syncthreads();
+    }
+    end();
+  }
+  if (!STATE && gr.last) {
+    // the rows' shares of dD and dbias meet in LDS
+    const size_t part = (size_t)at.b * p.S + at.s;
     __syncthreads();
     float* const red = lds;   // [2][ROWS][64]
+    if (wave >= W) {
 #pragma unroll
-    for (int i = 0; i < V; ++i) {
-      red[tr * SSM_CH + tc + i] = dD[i];
-      red[(Split::ROWS + tr) * SSM_CH + tc + i] = dbias[i];
+      for (int i = 0; i < V; ++i) {
+        red[row * SSM_CH + tc + i] = dD[i];
+        red[(SSM_ROWS + row) * SSM_CH + tc + i] = dbias[i];
+      }
     }
     __syncthreads();
-    for (int i = tid; i < 2 * SSM_CH; i += 64 * W) {
+    for (int i = threadIdx.x; i < 2 * SSM_CH; i += blockDim.x) {
       const int which = i / SSM_CH, ch = i % SSM_CH;
       float sum = 0.f;
-      for (int r = 0; r < Split::ROWS; ++r) sum += red[(which * Split::ROWS + r) * SSM_CH + ch];
+      for (int r = 0; r < SSM_ROWS; ++r) sum += red[(which * SSM_ROWS + r) * SSM_CH + ch];
       if (ch < at.cols) gr.part_d[(part * 2 + which) * E + at.c0 + ch] = sum;
     }
   }
 }
 
-template <typename T, int W, int NP, bool VEC>
+template <typename T, int W, bool VEC>
 hipError_t bwd_launch(const Ssm& p, const SsmGrad& gr, hipStream_t st) {
   const int nblk = p.G * p.gblocks;
+  const dim3 block(64 * (W + SSM_HELPERS));
   if (p.S > 1) {
-    constexpr int bytes = 3 * SSM_TILE * 4;
-    hipLaunchKernelGGL((ssm_bwd_kernel<T, W, NP, VEC, true>), dim3(nblk * (p.S - 1) * p.batch),
-                       dim3(64 * W), bytes, st, p, gr);
+    constexpr int bytes = ssm_bwd_lds<W, true>() * SSM_TILE * 4;
+    hipLaunchKernelGGL((ssm_bwd_kernel<T, W, VEC, true>), dim3(nblk * (p.S - 1) * p.batch), block,
+                       bytes, st, p, gr);
     if (hipError_t e = hipGetLastError(); e != hipSuccess) return e;
   }
-  constexpr int bytes = (3 + 3 * W) * SSM_TILE * 4;
-  if (hipError_t e = ensure_lds<ssm_bwd_kernel<T, W, NP, VEC, false>>(bytes); e != hipSuccess) return e;
-  hipLaunchKernelGGL((ssm_bwd_kernel<T, W, NP, VEC, false>), dim3(nblk * p.S * p.batch),
-                     dim3(64 * W), bytes, st, p, gr);
+  constexpr int bytes = ssm_bwd_lds<W, false>() * SSM_TILE * 4;
+  if (hipError_t e = ensure_lds<ssm_bwd_kernel<T, W, VEC, false>>(bytes); e != hipSuccess) return e;
+  hipLaunchKernelGGL((ssm_bwd_kernel<T, W, VEC, false>), dim3(nblk * p.S * p.batch), block, bytes, st,
+                     p, gr);
   return hipGetLastError();
 }
 
+// 16 states at a time: the first launches leave their sums over n in memory for the last
 template <typename T, bool VEC>
-hipError_t bwd_waves(const Ssm& p, const SsmGrad& gr, hipStream_t st) {
-  switch (ssm_waves(p.N)) {
-    case 1: return bwd_launch<T, 1, 1, VEC>(p, gr, st);
-    case 2: return bwd_launch<T, 2, 1, VEC>(p, gr, st);
-    case 4: return bwd_launch<T, 4, 1, VEC>(p, gr, st);
-    default:
-      return ssm_passes(p.N) == 1 ? bwd_launch<T, 8, 1, VEC>(p, gr, st)
-                                  : bwd_launch<T, 8, 2, VEC>(p, gr, st);
+hipError_t bwd_waves(const Ssm& p, SsmGrad gr, hipStream_t st) {
+  for (gr.n0 = 0; gr.n0 < p.N; gr.n0 += SSM_BWD_STATES) {
+    const int n = p.N - gr.n0;
+    gr.first = gr.n0 == 0;
+    gr.last = n <= SSM_BWD_STATES;
+    const hipError_t e = n <= 4   ? bwd_launch<T, 1, VEC>(p, gr, st)
+                         : n <= 8 ? bwd_launch<T, 2, VEC>(p, gr, st)
+                                  : bwd_launch<T, 4, VEC>(p, gr, st);
+    if (e != hipSuccess) return e;
   }
+  return hipSuccess;
 }
 
 hipError_t launch_ssm_bwd(const Ssm& p, const SsmGrad& gr, void* dB, void* dC, float* dA,
@@ -402,7 +442,7 @@ hipError_t launch_ssm_bwd(const Ssm& p, const SsmGrad& gr, void* dB, void* dC, f
                  : vec   ? bwd_waves<float, true>(p, gr, st)
                          : bwd_waves<float, false>(p, gr, st);
   if (e != hipSuccess) return e;
-  const int NQ = 4 * ssm_waves(p.N) * ssm_passes(p.N), parts = p.batch * p.S;
+  const int NQ = gr.NQ, parts = p.batch * p.S;
   const long long rows = (long long)p.batch * p.L;
   // dB and dC: the blocks of a group, for each group
   for (int g0 = 0; g0 < p.G; g0 += SUM_JOBS / 2) {
