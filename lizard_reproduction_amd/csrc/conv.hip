@@ -3,38 +3,42 @@
 //   pre_t = bias + sum_{j < K} w_j x_{t-K+1+j},   y_t = pre_t or silu(pre_t)
 //
 // K is at most four, so a value takes a few operations and the bytes of x and y (backward:
-// x, dy, y's recomputation and dx) bound it.  A thread takes eight channels and a run of
-// tokens, with the K rows in registers: a row is read once by the run it lies in and again,
-// from cache, by the run after it.  A workgroup's threads are columns of eight channels
+// x, dy, y's recomputation and dx) bound it.  A thread takes a vector of channels and a
+// run of tokens, with the K rows in registers: a row is read once by the run it lies in and again,
+// from cache, by the run after it.  A workgroup's threads are columns of vectors
 // times runs, a row's columns next to each other.
 //
 // Backward: g_t = dy_t act'(pre_t), dx_t = sum_j w_j g_{t+K-1-j} (the run goes K - 1 tokens
 // on), dw_j = sum_t g_t x_{t-K+1+j}, dbias = sum_t g_t: the workgroup's runs meet in LDS and
 // its shares go to a second launch, which adds them in order.
+#include <type_traits>
+
 #include "conv.hpp"
 
 namespace lz {
 
 // Where a thread works: its columns, and its run of tokens of a sequence
+template <int V, bool VEC>
 struct ConvPlace {
   int col, run, b, t0, left;
   bool in;
   __device__ __forceinline__ ConvPlace(const Conv& p) {
-    col = (blockIdx.y * p.cols + threadIdx.x % p.cols) * 8;
+    col = (blockIdx.y * p.cols + threadIdx.x % p.cols) * V;
     run = blockIdx.x * (CONV_THREADS / p.cols) + threadIdx.x / p.cols;
     in = col < p.C && run < p.batch * p.seq_runs;
     if (!in) col = 0, run = 0;
+    if (VEC && col + V > p.C) col = p.C - V;   // the last vector overlaps the one before
     b = run / p.seq_runs;
     t0 = (run - b * p.seq_runs) * p.run;
     left = p.C - col;
   }
 };
 
-template <int K>
-__device__ __forceinline__ void load_taps(const Conv& p, int col, int left, float (&w)[K][8],
-                                          float (&bias)[8]) {
+template <int K, int V>
+__device__ __forceinline__ void load_taps(const Conv& p, int col, int left, float (&w)[K][V],
+                                          float (&bias)[V]) {
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
+  for (int i = 0; i < V; ++i) {
     const int c = col + (i < left ? i : 0);
 #pragma unroll
     for (int j = 0; j < K; ++j) w[j][i] = p.w[(size_t)c * K + j];
@@ -43,44 +47,45 @@ __device__ __forceinline__ void load_taps(const Conv& p, int col, int left, floa
 }
 
 // Row t of sequence b, from the kept state where t < 0 (zeros without one)
-template <typename T, bool VEC, int K>
+template <typename T, bool VEC, int K, int V>
 __device__ __forceinline__ void row_before(const Conv& p, const T* xb, int b, int t, int col,
-                                           int left, float (&v)[8]) {
-  Cols8<T, VEC> c;
+                                           int left, float (&v)[V]) {
+  Cols<T, VEC, V> c;
   const T* state = (const T*)p.state_in;
   const bool have = t >= 0 || state;
   const T* from = t >= 0 || !state ? xb + (long long)max(t, 0) * p.x_t
                                    : state + ((long long)b * (K - 1) + (t + K - 1)) * p.C + col;
   c.load(from, left);
 #pragma unroll
-  for (int i = 0; i < 8; ++i) v[i] = have ? c.r.at(i) : 0.f;
+  for (int i = 0; i < V; ++i) v[i] = have ? c.r.at(i) : 0.f;
 }
 
 constexpr int CONV_AHEAD = 4;   // rows loaded before the first of them is used
 
 template <typename T, bool VEC, int K>
 __global__ __launch_bounds__(CONV_THREADS) void conv_fwd_kernel(Conv p) {
-  const ConvPlace at(p);
+  constexpr int V = CONV_FWD_V;
+  const ConvPlace<V, VEC> at(p);
   if (!at.in) return;
   const int len = p.lengths ? max(0, min(p.L, p.lengths[at.b])) : p.L;
   const T* xb = (const T*)p.x + at.b * p.x_b + at.col;
   T* yb = (T*)p.y + (long long)at.b * p.L * p.C + at.col;
-  float w[K][8], bias[8], win[K][8];   // win[j]: row t - K + 1 + j
-  load_taps<K>(p, at.col, at.left, w, bias);
+  float w[K][V], bias[V], win[K][V];   // win[j]: row t - K + 1 + j
+  load_taps<K, V>(p, at.col, at.left, w, bias);
 #pragma unroll
   for (int j = 1; j < K; ++j)
-    row_before<T, VEC, K>(p, xb, at.b, at.t0 + j - K, at.col, at.left, win[j]);
+    row_before<T, VEC, K, V>(p, xb, at.b, at.t0 + j - K, at.col, at.left, win[j]);
   const int t1 = min(at.t0 + p.run, p.L);
   for (int t = at.t0; t < t1; t += CONV_AHEAD) {
-    Cols8<T, VEC> next[CONV_AHEAD];
+    Cols<T, VEC, V> next[CONV_AHEAD];
 #pragma unroll
     for (int i = 0; i < CONV_AHEAD; ++i)
       next[i].load(xb + (long long)min(t + i, p.L - 1) * p.x_t, at.left);
 #pragma unroll
     for (int i = 0; i < CONV_AHEAD; ++i) {
-      Cols8<T, VEC> out;
+      Cols<T, VEC, V> out;
 #pragma unroll
-      for (int c = 0; c < 8; ++c) {
+      for (int c = 0; c < V; ++c) {
 #pragma unroll
         for (int j = 0; j + 1 < K; ++j) win[j][c] = win[j + 1][c];
         win[K - 1][c] = next[i].r.at(c);
@@ -97,11 +102,11 @@ __global__ __launch_bounds__(CONV_THREADS) void conv_fwd_kernel(Conv p) {
   if (K > 1 && p.state_out && at.t0 == 0) {
 #pragma unroll
     for (int j = 0; j < K - 1; ++j) {
-      float v[8];
-      row_before<T, VEC, K>(p, xb, at.b, len - (K - 1) + j, at.col, at.left, v);
-      Cols8<T, VEC> out;
+      float v[V];
+      row_before<T, VEC, K, V>(p, xb, at.b, len - (K - 1) + j, at.col, at.left, v);
+      Cols<T, VEC, V> out;
 #pragma unroll
-      for (int c = 0; c < 8; ++c) out.r.set(c, v[c]);
+      for (int c = 0; c < V; ++c) out.r.set(c, v[c]);
       out.store((T*)p.state_out + ((long long)at.b * (K - 1) + j) * p.C + at.col, at.left);
     }
   }
@@ -129,66 +134,77 @@ __global__ __launch_bounds__(256) void conv_step_kernel(Conv p) {
 template <typename T, bool VEC, int K>
 __global__ __launch_bounds__(CONV_THREADS) void conv_bwd_kernel(Conv p, const void* dy_, void* dx_,
                                                                 float* part) {
-  __shared__ float red[CONV_THREADS][9];
-  const ConvPlace at(p);
+  constexpr int V = CONV_BWD_V;
+  __shared__ float red[CONV_THREADS][V + 1];
+  const ConvPlace<V, VEC> at(p);
   const T* xb = (const T*)p.x + at.b * p.x_b + at.col;
   const T* dyb = (const T*)dy_ + (long long)at.b * p.L * p.C + at.col;
   T* dxb = (T*)dx_ + (long long)at.b * p.L * p.C + at.col;
-  float w[K][8], bias[8], win[K][8], g[K][8];   // g[j]: the gradient at token t - K + 1 + j
-  float dw[K][8], dbias[8];
-  load_taps<K>(p, at.col, at.left, w, bias);
+  float w[K][V], bias[V], win[K][V], g[K][V];   // g[j]: the gradient at token t - K + 1 + j
+  float dw[K][V], dbias[V];
+  load_taps<K, V>(p, at.col, at.left, w, bias);
 #pragma unroll
-  for (int c = 0; c < 8; ++c) {
+  for (int c = 0; c < V; ++c) {
     dbias[c] = 0.f;
 #pragma unroll
     for (int j = 0; j < K; ++j) dw[j][c] = g[j][c] = 0.f;
   }
 #pragma unroll
   for (int j = 1; j < K; ++j)
-    row_before<T, VEC, K>(p, xb, at.b, at.t0 + j - K, at.col, at.left, win[j]);
-  const int t1 = at.in ? min(at.t0 + p.run, p.L) : at.t0;   // the run's tokens,
-  const int t2 = at.in ? t1 + K - 1 : at.t0;                // and those their dx comes from
-  for (int t = at.t0; t < t2; t += CONV_AHEAD) {
-    Cols8<T, VEC> next[CONV_AHEAD], dy[CONV_AHEAD];
+    row_before<T, VEC, K, V>(p, xb, at.b, at.t0 + j - K, at.col, at.left, win[j]);
+  // Token t's row: its gradient g, this run's share of dw and dbias (OWN), and dx of token
+  // t - K + 1, the last whose taps are complete.  Past the sequence g is zero.
+  const int t1 = at.in ? min(at.t0 + p.run, p.L) : at.t0;
+  auto row = [&](int t, const Cols<T, VEC, V>& x, const Cols<T, VEC, V>& dy, auto own) {
+    Cols<T, VEC, V> out;
+    const bool there = t < p.L;
 #pragma unroll
-    for (int i = 0; i < CONV_AHEAD; ++i) {
-      const long long row = min(t + i, p.L - 1);
-      next[i].load(xb + row * p.x_t, at.left);
-      dy[i].load(dyb + row * p.C, at.left);
-    }
+    for (int c = 0; c < V; ++c) {
 #pragma unroll
-    for (int i = 0; i < CONV_AHEAD; ++i) {
-      Cols8<T, VEC> out;
-      const bool own = t + i < t1, there = t + i < p.L;
+      for (int j = 0; j + 1 < K; ++j) win[j][c] = win[j + 1][c], g[j][c] = g[j + 1][c];
+      win[K - 1][c] = x.r.at(c);
+      float d = dy.r.at(c);
+      if (p.act) {
+        float pre = bias[c];
 #pragma unroll
-      for (int c = 0; c < 8; ++c) {
-#pragma unroll
-        for (int j = 0; j + 1 < K; ++j) win[j][c] = win[j + 1][c], g[j][c] = g[j + 1][c];
-        win[K - 1][c] = next[i].r.at(c);
-        float d = dy[i].r.at(c);
-        if (p.act) {
-          float pre = bias[c];
-#pragma unroll
-          for (int j = 0; j < K; ++j) pre = fmaf(w[j][c], win[j][c], pre);
-          const float s = sigmoid(pre);
-          d *= s * fmaf(pre, 1.f - s, 1.f);
-        }
-        d = there ? d : 0.f;
-        g[K - 1][c] = d;
-        const float mine = own ? d : 0.f;
-        dbias[c] += mine;
-        float dx = 0.f;
-#pragma unroll
-        for (int j = 0; j < K; ++j) {
-          dw[j][c] = fmaf(mine, own ? win[j][c] : 0.f, dw[j][c]);
-          dx = fmaf(w[j][c], g[K - 1 - j][c], dx);   // g at token t - j: tap K - 1 - j
-        }
-        out.r.set(c, dx);
+        for (int j = 0; j < K; ++j) pre = fmaf(w[j][c], win[j][c], pre);
+        const float s = sigmoid(pre);
+        d *= s * fmaf(pre, 1.f - s, 1.f);
       }
-      (void)out;
-      if (t + i - (K - 1) >= at.t0 && t + i - (K - 1) < t1)
-        out.store(dxb + (long long)(t + i - (K - 1)) * p.C, at.left);
+      d = there ? d : 0.f;
+      g[K - 1][c] = d;
+      if (decltype(own)::value) dbias[c] += d;
+      float dx = 0.f;
+#pragma unroll
+      for (int j = 0; j < K; ++j) {
+        if (decltype(own)::value) dw[j][c] = fmaf(d, win[j][c], dw[j][c]);
+        dx = fmaf(w[j][c], g[K - 1 - j][c], dx);   // g at token t - j: tap K - 1 - j
+      }
+      out.r.set(c, dx);
     }
+    const int to = t - (K - 1);
+    if (to >= at.t0 && to < t1) out.store(dxb + (long long)to * p.C, at.left);
+  };
+  auto load = [&](int t, Cols<T, VEC, V>& x, Cols<T, VEC, V>& dy) {
+    const long long r = min(t, p.L - 1);
+    x.load(xb + r * p.x_t, at.left);
+    dy.load(dyb + r * p.C, at.left);
+  };
+  // A run is whole batches of rows, but the last one, whose rows past it are past the sequence
+  int t = at.t0;
+  for (; t < t1; t += CONV_AHEAD) {
+    Cols<T, VEC, V> x[CONV_AHEAD], dy[CONV_AHEAD];
+#pragma unroll
+    for (int i = 0; i < CONV_AHEAD; ++i) load(t + i, x[i], dy[i]);
+#pragma unroll
+    for (int i = 0; i < CONV_AHEAD; ++i) row(t + i, x[i], dy[i], std::true_type());
+  }
+  if (K > 1 && at.in) {   // the tokens after the run that its last rows reach
+    Cols<T, VEC, V> x[K], dy[K];
+#pragma unroll
+    for (int i = 0; i < K - 1; ++i) load(t + i, x[i], dy[i]);
+#pragma unroll
+    for (int i = 0; i < K - 1; ++i) row(t + i, x[i], dy[i], std::false_type());
   }
   // the workgroup's runs, one sum at a time: [K + 1][C] floats a row of workgroups
   const int runs = CONV_THREADS / p.cols;
@@ -196,13 +212,17 @@ __global__ __launch_bounds__(CONV_THREADS) void conv_bwd_kernel(Conv p, const vo
   for (int j = 0; j <= K; ++j) {
     __syncthreads();
 #pragma unroll
-    for (int c = 0; c < 8; ++c) red[threadIdx.x][c] = j < K ? dw[j < K ? j : 0][c] : dbias[c];
+    for (int c = 0; c < V; ++c) red[threadIdx.x][c] = j < K ? dw[j < K ? j : 0][c] : dbias[c];
     __syncthreads();
-    for (int i = threadIdx.x; i < 8 * p.cols; i += CONV_THREADS) {
-      const int ch = blockIdx.y * p.cols * 8 + i;
+    for (int i = threadIdx.x; i < V * p.cols; i += CONV_THREADS) {
+      const int t = i / V;   // the threads of a column of vectors
+      int ch = (blockIdx.y * p.cols + t) * V;
+      if (ch >= p.C) continue;
+      if (VEC && ch + V > p.C) ch = p.C - V;
+      ch += i % V;
       if (ch >= p.C) continue;
       float sum = 0.f;
-      for (int r = 0; r < runs; ++r) sum += red[r * p.cols + i / 8][i % 8];
+      for (int r = 0; r < runs; ++r) sum += red[r * p.cols + t][i % V];
       part[((size_t)blockIdx.x * (K + 1) + j) * p.C + ch] = sum;
     }
   }
@@ -210,8 +230,8 @@ __global__ __launch_bounds__(CONV_THREADS) void conv_bwd_kernel(Conv p, const vo
 
 // Runs long enough that their K - 1 rows before them cost little, short enough that the
 // threads fill the chip twice over
-void conv_split(Conv& p) {
-  const int vecs = (p.C + 7) / 8;
+void conv_split(Conv& p, bool backward) {
+  const int V = backward ? CONV_BWD_V : CONV_FWD_V, vecs = (p.C + V - 1) / V;
   int cols = 1;
   while (cols < 64 && cols < vecs) cols *= 2;
   p.cols = cols;

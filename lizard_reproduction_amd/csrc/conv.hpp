@@ -5,6 +5,7 @@
 namespace lz {
 
 constexpr int CONV_THREADS = 256, CONV_MAX_TAPS = 4;
+constexpr int CONV_FWD_V = 8, CONV_BWD_V = 4;   // channels a thread
 
 struct Conv {
   const void* x;
@@ -16,11 +17,11 @@ struct Conv {
   long long x_b;                 // elements from one sequence to the next
   int x_t;                       // and from one token to the next
   int batch, L, C, act;
-  // conv_split: columns (of eight channels) a workgroup, tokens a run, runs a sequence
+  // conv_split: columns (vectors of channels) a workgroup, tokens a run, runs a sequence
   int cols, col_blocks, run, seq_runs, run_blocks;
 };
 
-void conv_split(Conv& p);
+void conv_split(Conv& p, bool backward);
 hipError_t launch_conv(const Conv& p, int K, const void* dy, void* dx, float* part, bool is_bf16,
                        bool vec, hipStream_t st);
 hipError_t launch_conv_sums(const Conv& p, int K, const float* part, float* dw, float* dbias,

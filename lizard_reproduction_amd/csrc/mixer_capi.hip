@@ -217,18 +217,11 @@ int check_conv(const char* what, const void* x, const float* w, long long batch,
   return fail(1, "%s: null input pointer", what);
 }
 
-lz::Conv conv_of(int batch, int length, int channels) {
+lz::Conv conv_of(int batch, int length, int channels, bool backward = false) {
   lz::Conv p = {};
   p.batch = batch, p.L = length, p.C = channels;
-  lz::conv_split(p);
+  lz::conv_split(p, backward);
   return p;
-}
-
-bool conv_vec(const lz::Conv& p, std::initializer_list<const void*> rows) {
-  if (p.C % 8 || p.x_b % 8 || p.x_t % 8 || !aligned(p.x, 16)) return false;
-  for (const void* r : rows)
-    if (!aligned(r, 16)) return false;
-  return true;
 }
 
 }  // namespace
@@ -245,7 +238,7 @@ extern "C" int lz_short_conv_fwd(const void* x, long long x_batch, long long x_t
   p.x = x, p.w = weight, p.bias = bias, p.state_in = state_in, p.state_out = state_out;
   p.lengths = lengths, p.y = y, p.x_b = x_batch, p.x_t = (int)x_token, p.act = silu;
   return hip_status(lz::launch_conv(p, taps, nullptr, nullptr, nullptr, bf16 != 0,
-                                    conv_vec(p, {y, state_in, state_out}), (hipStream_t)stream),
+                                    channels >= lz::CONV_FWD_V, (hipStream_t)stream),
                     "short_conv_fwd");
 }
 
@@ -264,7 +257,7 @@ extern "C" int lz_short_conv_decode_step(const void* x, long long x_batch, const
 
 extern "C" size_t lz_short_conv_bwd_workspace_bytes(int batch, int length, int channels, int taps) {
   if (batch <= 0 || length <= 0 || channels <= 0 || taps <= 0) return 0;
-  return (size_t)conv_of(batch, length, channels).run_blocks * (taps + 1) * channels * 4;
+  return (size_t)conv_of(batch, length, channels, true).run_blocks * (taps + 1) * channels * 4;
 }
 
 extern "C" int lz_short_conv_bwd(const void* x, long long x_batch, long long x_token,
@@ -275,13 +268,13 @@ extern "C" int lz_short_conv_bwd(const void* x, long long x_batch, long long x_t
   if (int rc = check_conv("short_conv_bwd", x, weight, batch, length, channels, taps, x_batch, x_token))
     return rc;
   if (!dy || !dx || !dweight) return fail(1, "short_conv_bwd: null pointer");
-  lz::Conv p = conv_of(batch, length, channels);
+  lz::Conv p = conv_of(batch, length, channels, true);
   p.x = x, p.w = weight, p.bias = bias, p.x_b = x_batch, p.x_t = (int)x_token, p.act = silu;
   const size_t need = lz_short_conv_bwd_workspace_bytes(batch, length, channels, taps);
   if (!workspace || workspace_bytes < need)
     return fail(1, "short_conv_bwd: workspace of %zu bytes given, %zu needed", workspace_bytes, need);
   hipError_t e = lz::launch_conv(p, taps, dy, dx, (float*)workspace, bf16 != 0,
-                                 conv_vec(p, {dy, dx}), (hipStream_t)stream);
+                                 channels >= lz::CONV_BWD_V, (hipStream_t)stream);
   if (e == hipSuccess)
     e = lz::launch_conv_sums(p, taps, (const float*)workspace, dweight, dbias, (hipStream_t)stream);
   return hip_status(e, "short_conv_bwd");
@@ -324,19 +317,13 @@ lz::Norm norm_of(const lz_group_norm_args* a, bool backward) {
   p.z_b = a->gate_batch, p.z_t = a->gate_token, p.z_g = a->gate_group;
   p.batch = a->batch, p.L = a->length, p.G = a->groups, p.W = a->width, p.act = a->silu;
   p.eps = a->eps;
+  // sequences that follow each other in every tensor are one
+  if (p.x_b == p.L * p.x_t && (!p.gate || p.z_b == p.L * p.z_t)) {
+    p.L *= p.batch;
+    p.batch = 1;
+  }
   lz::norm_split(p, backward);
   return p;
-}
-
-bool norm_vec(const lz::Norm& p, std::initializer_list<const void*> rows) {
-  if (p.W % 8) return false;
-  for (long long s : {p.x_b, p.x_t, p.x_g})
-    if (s % 8) return false;
-  for (long long s : {p.z_b, p.z_t, p.z_g})
-    if (p.gate && s % 8) return false;
-  for (const void* r : rows)
-    if (!aligned(r, 16)) return false;
-  return aligned(p.x, 16) && aligned(p.gate, 16);
 }
 
 }  // namespace
@@ -346,7 +333,7 @@ extern "C" int lz_group_norm_fwd(const lz_group_norm_args* args, void* y, void* 
   if (!y) return fail(1, "group_norm_fwd: null output pointer");
   lz::Norm p = norm_of(args, false);
   p.y = y;
-  return hip_status(lz::launch_norm_fwd(p, args->bf16 != 0, norm_vec(p, {y}), (hipStream_t)stream),
+  return hip_status(lz::launch_norm_fwd(p, args->bf16 != 0, (hipStream_t)stream),
                     "group_norm_fwd");
 }
 
@@ -370,7 +357,6 @@ extern "C" int lz_group_norm_bwd(const lz_group_norm_args* args, const void* dy,
   if (need && (!workspace || workspace_bytes < need))
     return fail(1, "group_norm_bwd: workspace of %zu bytes given, %zu needed", workspace_bytes, need);
   return hip_status(lz::launch_norm_bwd(p, dy, dx, dgate, need ? (float*)workspace : nullptr,
-                                        dweight, dbias, args->bf16 != 0,
-                                        norm_vec(p, {dy, dx, dgate}), (hipStream_t)stream),
+                                        dweight, dbias, args->bf16 != 0, (hipStream_t)stream),
                     "group_norm_bwd");
 }

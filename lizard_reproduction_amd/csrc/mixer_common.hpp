@@ -98,22 +98,31 @@ __device__ __forceinline__ void store_raw(rsrc_t r, uint32_t off, bool in, int l
   }
 }
 
-// Eight channels of a row through a pointer of the lane's own.  Rows are clamped into the
+// N channels of a row through a pointer of the lane's own, as vectors of up to 16 bytes at
+// any alignment (VEC), else element by element, `left` of them.  Rows are clamped into the
 // tensor by the callers and what does not exist is selected away after the load, so no
 // branch holds loads apart.
-template <typename T, bool VEC>
-struct Cols8 {
-  RawRow<T, 8, VEC> r;
+typedef uint32_t u32x4_any __attribute__((ext_vector_type(4), aligned(2)));
+typedef uint32_t u32x2_any __attribute__((ext_vector_type(2), aligned(2)));
+
+template <typename T, bool VEC, int N>
+struct Cols {
+  RawRow<T, N, VEC> r;
+  static constexpr int BYTES = N * (int)sizeof(T);
   __device__ __forceinline__ void load(const T* p, int left) {
-    if constexpr (VEC) {
+    if constexpr (VEC && BYTES == 8) {
+      const u32x2_any v = *reinterpret_cast<const u32x2_any*>(p);
+      r.w[0] = v[0], r.w[1] = v[1];
+    } else if constexpr (VEC) {
 #pragma unroll
-      for (int k = 0; k < (int)sizeof(T) / 2; ++k) {
-        const uint4 v = reinterpret_cast<const uint4*>(p)[k];
-        r.w[4 * k] = v.x, r.w[4 * k + 1] = v.y, r.w[4 * k + 2] = v.z, r.w[4 * k + 3] = v.w;
+      for (int k = 0; k < BYTES / 16; ++k) {
+        const u32x4_any v = reinterpret_cast<const u32x4_any*>(p)[k];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) r.w[4 * k + i] = v[i];
       }
     } else {
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
+      for (int i = 0; i < N; ++i) {
         const T v = p[i < left ? i : 0];
         if constexpr (IS_BF16<T>) r.w[i] = __builtin_bit_cast(uint16_t, v);
         else r.w[i] = __builtin_bit_cast(uint32_t, v);
@@ -121,14 +130,16 @@ struct Cols8 {
     }
   }
   __device__ __forceinline__ void store(T* p, int left) const {
-    if constexpr (VEC) {
+    if constexpr (VEC && BYTES == 8) {
+      *reinterpret_cast<u32x2_any*>(p) = u32x2_any{r.w[0], r.w[1]};
+    } else if constexpr (VEC) {
 #pragma unroll
-      for (int k = 0; k < (int)sizeof(T) / 2; ++k)
-        reinterpret_cast<uint4*>(p)[k] =
-            uint4{r.w[4 * k], r.w[4 * k + 1], r.w[4 * k + 2], r.w[4 * k + 3]};
+      for (int k = 0; k < BYTES / 16; ++k)
+        reinterpret_cast<u32x4_any*>(p)[k] =
+            u32x4_any{r.w[4 * k], r.w[4 * k + 1], r.w[4 * k + 2], r.w[4 * k + 3]};
     } else {
 #pragma unroll
-      for (int i = 0; i < 8; ++i)
+      for (int i = 0; i < N; ++i)
         if (i < left) p[i] = (T)r.at(i);
     }
   }
@@ -174,8 +185,38 @@ __device__ __forceinline__ float dpp(float x) {
       float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, x), CTRL, 0xf, 0xf, true));
 }
 constexpr int DPP_XOR1 = 0xb1, DPP_XOR2 = 0x4e;          // quad_perm [1,0,3,2], [2,3,0,1]
-constexpr int DPP_HALF_MIRROR = 0x141, DPP_ROR8 = 0x128; // lane 7 - i of its 8; lane i + 8 mod 16
+constexpr int DPP_HALF_MIRROR = 0x141, DPP_MIRROR = 0x140;   // lane 7 - i of its 8, 15 - i of its 16
+constexpr int DPP_ROR8 = 0x128;                          // lane i + 8 mod 16
 constexpr int DPP_BCAST = 0x150;                         // + k: lane k of the row, to all of it
+
+// a + b of the two registers that a swap of a's and b's half waves (rows of 16) leaves:
+// the swapped halves next to each other, each with what the other register held of it.
+// (The swap's results are copied out first: a bit cast of an element of its vector reads
+// element 0.)
+template <bool ROWS>
+__device__ __forceinline__ float swap_add(float a, float b) {
+  const uint32_t x = __builtin_bit_cast(uint32_t, a), y = __builtin_bit_cast(uint32_t, b);
+  uint32_t lo, hi;
+  if constexpr (ROWS) {
+    const auto s = __builtin_amdgcn_permlane16_swap(x, y, false, false);
+    lo = s[0], hi = s[1];
+  } else {
+    const auto s = __builtin_amdgcn_permlane32_swap(x, y, false, false);
+    lo = s[0], hi = s[1];
+  }
+  return __builtin_bit_cast(float, lo) + __builtin_bit_cast(float, hi);
+}
+
+// The sum over each `lanes` (a power of two, uniform) consecutive lanes, in all of them
+__device__ __forceinline__ float lanes_sum(float v, int lanes) {
+  if (lanes > 1) v += dpp<DPP_XOR1>(v);
+  if (lanes > 2) v += dpp<DPP_XOR2>(v);
+  if (lanes > 4) v += dpp<DPP_HALF_MIRROR>(v);
+  if (lanes > 8) v += dpp<DPP_MIRROR>(v);
+  if (lanes > 16) v = swap_add<true>(v, v);
+  if (lanes > 32) v = swap_add<false>(v, v);
+  return v;
+}
 
 // Sums of partial results in the order of their index, by one launch.  A job sums, for
 // each of `rows` x `cols` outputs, `parts` values `part_stride` floats apart that begin

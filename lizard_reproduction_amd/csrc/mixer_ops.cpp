@@ -204,6 +204,55 @@ Tensor ssm_step(const Tensor& x, const Tensor& dt, const Tensor& A, const Tensor
   return y.to(x.scalar_type());
 }
 
+// Whether a decode step's launch takes t as it is: on x's device, of the given type and
+// sizes, its last dimension contiguous (all of it, with whole)
+bool fits(const Tensor& t, const Tensor& x, at::ScalarType dtype, at::IntArrayRef sizes, bool whole) {
+  const int64_t last = t.dim() - 1;
+  return t.is_cuda() && t.device() == x.device() && t.scalar_type() == dtype &&
+         t.sizes() == sizes && (whole ? t.is_contiguous() : t.size(last) == 1 || t.stride(last) == 1);
+}
+bool fits(const Opt& t, const Tensor& x, at::ScalarType dtype, at::IntArrayRef sizes, bool whole) {
+  return !t || fits(*t, x, dtype, sizes, whole);
+}
+// x's own form, and a state that may be written in place
+bool fits_step(const Tensor& x, const Tensor& state) {
+  return x.dim() == 2 && x.is_cuda() && x.numel() && x.numel() < (1LL << 31) &&
+         (x.scalar_type() == at::kBFloat16 || x.scalar_type() == at::kFloat) &&
+         (x.size(1) == 1 || x.stride(1) == 1) &&
+         !(at::GradMode::is_enabled() && state.requires_grad());
+}
+
+// The step of operands that its launch takes as they are, checked here once and not in
+// Python (a step of one sequence: 17 -> 8 us, its kernel takes 3); no output for others,
+// which go through ssm_step after Python's checks.
+Opt ssm_step_direct(const Tensor& x, const Tensor& dt, const Tensor& A, const Tensor& B,
+                    const Tensor& C, const Tensor& state, const Opt& D, const Opt& z,
+                    const Opt& bias, bool softplus) {
+  if (!fits_step(x, state) || A.dim() != 2 || (B.dim() != 2 && B.dim() != 3)) return {};
+  const auto t = x.scalar_type();
+  const int64_t b = x.size(0), e = x.size(1), n = A.size(1), g = B.dim() == 3 ? B.size(1) : 1;
+  const auto bc = B.dim() == 3 ? std::vector<int64_t>{b, g, n} : std::vector<int64_t>{b, n};
+  if (n < 1 || n > LZ_SSM_MAX_STATE || g < 1 || e % g || !fits(dt, x, t, {b, e}, false) ||
+      !fits(A, x, at::kFloat, {e, n}, true) || !fits(B, x, t, bc, false) ||
+      !fits(C, x, t, bc, false) || !fits(state, x, at::kFloat, {b, e, n}, true) ||
+      !fits(D, x, at::kFloat, {e}, true) || !fits(z, x, t, {b, e}, false) ||
+      !fits(bias, x, at::kFloat, {e}, true))
+    return {};
+  const c10::DeviceGuard guard(x.device());
+  const Tensor y = at::empty({b, e}, x.options());
+  lz_ssm_args a = {};
+  a.x = ptr(x), a.dt = ptr(dt), a.z = z ? ptr(*z) : nullptr, a.B = ptr(B), a.C = ptr(C);
+  a.A = ptr<float>(A), a.D = D ? ptr<float>(*D) : nullptr;
+  a.dt_bias = bias ? ptr<float>(*bias) : nullptr;
+  a.x_batch = step_of(x, 0), a.dt_batch = step_of(dt, 0), a.z_batch = z ? step_of(*z, 0) : 0;
+  a.B_batch = step_of(B, 0), a.C_batch = step_of(C, 0);
+  if (B.dim() == 3) a.B_group = step_of(B, 1), a.C_group = step_of(C, 1);
+  a.batch = i32(b), a.channels = i32(e), a.state = i32(n), a.groups = i32(g);
+  a.softplus = softplus, a.bf16 = t == at::kBFloat16;
+  check(lz_ssm_decode_step(&a, ptr<float>(state), ptr(y), stream_of(x)), "lz_ssm_decode_step");
+  return y;
+}
+
 // ---------------------------------------------------------------------------
 // short causal convolution
 // ---------------------------------------------------------------------------
@@ -300,6 +349,24 @@ Tensor short_conv_step(const Tensor& x, const Tensor& w, const Tensor& state, co
   return y;
 }
 
+// as ssm_step_direct
+Opt short_conv_step_direct(const Tensor& x, const Tensor& w, const Tensor& state, const Opt& bias,
+                           bool silu) {
+  if (!fits_step(x, state) || w.dim() != 2) return {};
+  const int64_t b = x.size(0), c = x.size(1), k = w.size(1);
+  if (k < 1 || k > LZ_CONV_MAX_TAPS || !fits(w, x, at::kFloat, {c, k}, true) ||
+      !fits(state, x, x.scalar_type(), {b, k - 1, c}, true) || !fits(bias, x, at::kFloat, {c}, true))
+    return {};
+  const c10::DeviceGuard guard(x.device());
+  const Tensor y = at::empty({b, c}, x.options());
+  check(lz_short_conv_decode_step(ptr(x), step_of(x, 0), ptr<float>(w),
+                                  bias ? ptr<float>(*bias) : nullptr, ptr(state), ptr(y), i32(b),
+                                  i32(c), i32(k), silu, x.scalar_type() == at::kBFloat16,
+                                  stream_of(x)),
+        "lz_short_conv_decode_step");
+  return y;
+}
+
 // ---------------------------------------------------------------------------
 // group norm
 // ---------------------------------------------------------------------------
@@ -392,6 +459,8 @@ void bind_mixers(py::module_& m) {
   m.def("ssm", &ssm, nogil);
   m.def("ssm_prefill", &ssm_prefill, nogil);
   m.def("ssm_step", &ssm_step, nogil);
+  m.def("ssm_step_direct", &ssm_step_direct, nogil);
+  m.def("short_conv_step_direct", &short_conv_step_direct, nogil);
   m.def("short_conv", &short_conv, nogil);
   m.def("short_conv_prefill", &short_conv_prefill, nogil);
   m.def("short_conv_step", &short_conv_step, nogil);

@@ -13,14 +13,14 @@ struct Norm {
   long long x_b, x_t, x_g;       // elements from one sequence, token and group to the next
   long long z_b, z_t, z_g;       // of the gate
   int batch, L, G, W, act;       // act: silu of the result (or of the gate), else neither
-  float eps;
+  float eps, inv_w;
   // norm_split: threads and vectors a group, groups and rows a workgroup, its grid
   int tpg, vecs, gb, rb, group_blocks, row_blocks;
 };
 
 void norm_split(Norm& p, bool backward);
-hipError_t launch_norm_fwd(const Norm& p, bool is_bf16, bool vec, hipStream_t st);
+hipError_t launch_norm_fwd(const Norm& p, bool is_bf16, hipStream_t st);
 hipError_t launch_norm_bwd(const Norm& p, const void* dy, void* dx, void* dgate, float* part,
-                           float* dw, float* dbias, bool is_bf16, bool vec, hipStream_t st);
+                           float* dw, float* dbias, bool is_bf16, hipStream_t st);
 
 }  // namespace lz

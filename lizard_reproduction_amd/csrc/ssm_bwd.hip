@@ -20,24 +20,6 @@
 
 namespace lz {
 
-// a + b of the two registers that a swap of a's and b's half waves (rows of 16) leaves:
-// the swapped halves next to each other, each with what the other register held of it.
-// (The swap's results are copied out first: a bit cast of an element of its vector reads
-// element 0.)
-template <bool ROWS>
-__device__ __forceinline__ float swap_add(float a, float b) {
-  const uint32_t x = __builtin_bit_cast(uint32_t, a), y = __builtin_bit_cast(uint32_t, b);
-  uint32_t lo, hi;
-  if constexpr (ROWS) {
-    const auto s = __builtin_amdgcn_permlane16_swap(x, y, false, false);
-    lo = s[0], hi = s[1];
-  } else {
-    const auto s = __builtin_amdgcn_permlane32_swap(x, y, false, false);
-    lo = s[0], hi = s[1];
-  }
-  return __builtin_bit_cast(float, lo) + __builtin_bit_cast(float, hi);
-}
-
 // The sums of v0 .. v7 over the wave: lane l gets sum l / 8.
 __device__ __forceinline__ float wave_sums8(const float (&v)[8]) {
   float q[4], r[2];

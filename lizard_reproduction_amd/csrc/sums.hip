@@ -8,7 +8,7 @@
 
 namespace lz {
 
-constexpr int SUM_WAVES = 4, SUM_BATCH = 8;
+constexpr int SUM_WAVES = 8, SUM_BATCH = 8;
 
 struct SumGrid {
   SumJobs jobs;

@@ -600,7 +600,7 @@ def _check_activations(what, **tensors):
             raise ValueError(f"{what}: {name} is on {t.device}, the others on {device}")
         if t.dtype not in _ACTIVATIONS:
             raise ValueError(f"{what}: {name} must be bf16 or fp32, got {t.dtype}")
-        if t.numel() >= 2 ** 40 or any(n >= 2 ** 31 for n in t.shape):
+        if t.numel() >= 2 ** 31 and max(t.shape) >= 2 ** 31:
             raise ValueError(f"{what}: {name} {tuple(t.shape)} is too large")
     return device
 
@@ -643,6 +643,18 @@ def _check_state(what, state, shape, dtype, device, in_place=False):
                          f"{tuple(shape)} on {device}, got {got}")
     if in_place and state.requires_grad and torch.is_grad_enabled():
         raise ValueError(f"{what}: state is updated in place and may not require gradients")
+
+
+def _direct(name, *operands):
+    """A decode step whose operands its launch takes as they are (C++ checks
+    them); None for others, which the Python checks below refuse or cast."""
+    if not _gpu_present() or not _ops.plain():
+        return None
+    _refuse_capture("lizard_reproduction_amd kernels")
+    try:
+        return getattr(_ops.load(), name)(*operands)
+    except TypeError:     # an operand that is no tensor
+        return None
 
 
 def _silu(what, activation):
@@ -704,6 +716,10 @@ def short_conv_decode_step(x, weight, state, bias=None, activation="silu"):
     ``state`` (``[B, K - 1, C]`` in x's dtype, from ``short_conv_prefill`` or
     zeros) on by it, in place.  No autograd."""
     what = "short_conv_decode_step"
+    if activation in (None, "silu"):
+        y = _direct("short_conv_step_direct", x, weight, state, bias, activation == "silu")
+        if y is not None:
+            return y
     silu = _check_conv(what, x, weight, bias, activation, 2)
     _check_state(what, state, (x.shape[0], weight.shape[1] - 1, x.shape[1]), x.dtype, x.device, True)
     return _ops.load().short_conv_step(x[:, None], weight, state, bias, silu)[:, 0]
@@ -779,6 +795,9 @@ def ssm_decode_step(x, dt, A, B, C, state, D=None, z=None, dt_bias=None, dt_soft
     ``state`` (contiguous fp32 ``[B, E, N]``) in place.  x, dt, z ``[B, E]``;
     B, C ``[B, N]`` or ``[B, G, N]``.  Returns y ``[B, E]``; no autograd."""
     what = "ssm_decode_step"
+    y = _direct("ssm_step_direct", x, dt, A, B, C, state, D, z, dt_bias, bool(dt_softplus))
+    if y is not None:
+        return y
     B, C = _check_ssm(what, x, dt, A, B, C, D, z, dt_bias, True)
     _check_state(what, state, (x.shape[0], x.shape[1], A.shape[1]), torch.float32, x.device, True)
     if z is not None:
