@@ -429,8 +429,9 @@ typedef struct {
   int softplus, bf16;
 } lz_ssm_args;
 
-/* Bytes of the states lz_ssm_fwd keeps for lz_ssm_bwd (one every 16 tokens). */
-size_t lz_ssm_states_bytes(int batch, int length, int channels, int state);
+/* Bytes of what lz_ssm_fwd keeps for lz_ssm_bwd: states, one every 16 tokens, and with
+ * a gate (`gated`: z is given) the f32 rows that it multiplies. */
+size_t lz_ssm_states_bytes(int batch, int length, int channels, int state, int gated);
 /* Workspace bytes of lz_ssm_fwd: the segments' own states, 0 when the
  * sequences' channels alone fill the GPU. */
 size_t lz_ssm_fwd_workspace_bytes(int batch, int length, int channels, int state, int groups);

@@ -48,7 +48,7 @@ SIGNATURES = {
     "lz_layer_combine_fwd": (_I, [_P, _P, _P, _P, _I, _I, _I, _I, _I, _P]),
     "lz_layer_combine_bwd_workspace_bytes": (_S, []),
     "lz_layer_combine_bwd": (_I, [_P, _P, _P, _P, _P, _P, _I, _I, _I, _I, _I, _P, _S, _P]),
-    "lz_ssm_states_bytes": (_S, [_I, _I, _I, _I]),
+    "lz_ssm_states_bytes": (_S, [_I, _I, _I, _I, _I]),
     "lz_ssm_fwd_workspace_bytes": (_S, [_I, _I, _I, _I, _I]),
     "lz_ssm_fwd": (_I, [_P, _P, _P, _P, _P, _P, _P, _S, _P]),
     "lz_ssm_decode_step": (_I, [_P, _P, _P, _P]),

@@ -113,7 +113,13 @@ size_t ssm_part_bc(const lz::Ssm& p) {
 
 // Sums over n that pass from one launch to the next
 size_t ssm_acc(const lz::Ssm& p) {
-  return p.N > lz::SSM_BWD_STATES ? 3 * (size_t)p.batch * p.L * p.E : 0;
+  return p.N > lz::SSM_BWD_STATES ? 2 * (size_t)p.batch * p.L * p.E : 0;
+}
+
+// What the forward keeps for the backward: the rows that z gates, then the tiles' states
+void ssm_kept(lz::Ssm& p, float* states) {
+  p.mixed = p.z ? states : nullptr;
+  p.saved = states && p.z ? states + (size_t)p.batch * p.L * p.E : states;
 }
 
 bool ssm_sizes_ok(int batch, int length, int channels, int state, int groups) {
@@ -122,9 +128,10 @@ bool ssm_sizes_ok(int batch, int length, int channels, int state, int groups) {
 
 }  // namespace
 
-extern "C" size_t lz_ssm_states_bytes(int batch, int length, int channels, int state) {
+extern "C" size_t lz_ssm_states_bytes(int batch, int length, int channels, int state, int gated) {
   if (!ssm_sizes_ok(batch, length, channels, state, 1)) return 0;
-  return (size_t)batch * ((length + lz::SSM_TT - 1) / lz::SSM_TT) * channels * state * 4;
+  const size_t tiles = (length + lz::SSM_TT - 1) / lz::SSM_TT, rows = gated ? length : 0;
+  return (size_t)batch * channels * (rows + tiles * state) * 4;
 }
 
 extern "C" size_t lz_ssm_fwd_workspace_bytes(int batch, int length, int channels, int state,
@@ -143,7 +150,8 @@ extern "C" int lz_ssm_fwd(const lz_ssm_args* args, const float* state_in, float*
   const size_t need = ssm_records(p) * 4;
   if (need && (!workspace || workspace_bytes < need))
     return fail(1, "ssm_fwd: workspace of %zu bytes given, %zu needed", workspace_bytes, need);
-  p.state_in = state_in, p.state_out = state_out, p.lengths = lengths, p.y = y, p.saved = states;
+  p.state_in = state_in, p.state_out = state_out, p.lengths = lengths, p.y = y;
+  ssm_kept(p, states);
   p.rec = (float*)workspace;
   p.dsum = p.rec + (size_t)p.batch * (p.S - 1) * p.E * p.N;
   return hip_status(lz::launch_ssm_fwd(p, args->bf16 != 0, ssm_vec(p, args->bf16, {y}),
@@ -178,7 +186,7 @@ extern "C" int lz_ssm_bwd(const lz_ssm_args* args, const float* states, const vo
   const size_t need = lz_ssm_bwd_workspace_bytes(p.batch, p.L, p.E, p.N, p.G);
   if (!workspace || workspace_bytes < need)
     return fail(1, "ssm_bwd: workspace of %zu bytes given, %zu needed", workspace_bytes, need);
-  p.saved = const_cast<float*>(states);
+  ssm_kept(p, const_cast<float*>(states));
   lz::SsmGrad g = {};
   g.dy = dy, g.dx = dx, g.ddt = ddt, g.dz = dz;
   g.acc = (float*)workspace;

@@ -128,7 +128,7 @@ struct SsmNode : torch::autograd::Function<SsmNode> {
     const SsmCall c = ssm_call(x, dt, A, B, C, D, z, bias, softplus);
     const lz_ssm_args a = c.args();
     const Tensor states = at::empty(
-        {static_cast<int64_t>(lz_ssm_states_bytes(a.batch, a.length, a.channels, a.state) / 4)},
+        {static_cast<int64_t>(lz_ssm_states_bytes(a.batch, a.length, a.channels, a.state, a.z != nullptr) / 4)},
         c.A.options());
     const Tensor y = c.forward({}, {}, {}, states);
     ctx->save_for_backward({c.x, c.dt, c.A, c.B, c.C, c.D, c.z, c.bias});

@@ -202,7 +202,7 @@ __global__ __launch_bounds__(NORM_THREADS) void norm_fwd_kernel(Norm p) {
 }
 
 template <typename T, NormFit FIT, int N>
-__global__ __launch_bounds__(NORM_THREADS) void norm_bwd_kernel(Norm p, const void* dy_, void* dx_,
+__global__ __launch_bounds__(NORM_THREADS, N == 1 ? 4 : 1) void norm_bwd_kernel(Norm p, const void* dy_, void* dx_,
                                                                 void* dgate_, float* part) {
   __shared__ float red[4];
   __shared__ float shares[NORM_THREADS][9];

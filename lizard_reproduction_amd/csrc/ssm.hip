@@ -55,38 +55,50 @@ __global__ __launch_bounds__(64 * (W + SSM_HELPERS)) void ssm_fwd_kernel(Ssm p) 
     if (has_z) zb += SSM_TT * (long long)z_t;
   };
   auto prep = [&](int rows, int buf) {
-    {
-      float d[V], u[V];
+    float d[V], u[V];
 #pragma unroll
-      for (int i = 0; i < V; ++i) {
-        d[i] = dr.at(i) + bias[i];
-        if (soft) d[i] = softplus(d[i]);
-        if (row >= rows) d[i] = 0.f;   // past the length: the state stays as it is
-        u[i] = d[i] * xr.at(i);
-      }
-      put_row(sd[buf] + row * SSM_CH + tc, d);
-      put_row(su[buf] + row * SSM_CH + tc, u);
+    for (int i = 0; i < V; ++i) {
+      d[i] = dr.at(i) + bias[i];
+      if (soft) d[i] = softplus(d[i]);
+      u[i] = d[i] * xr.at(i);
     }
+    if (rows < SSM_TT && row >= rows) {   // past the length: the state stays as it is
+#pragma unroll
+      for (int i = 0; i < V; ++i) d[i] = u[i] = 0.f;
+    }
+    put_row(sd[buf] + row * SSM_CH + tc, d);
+    put_row(su[buf] + row * SSM_CH + tc, u);
   };
-  auto finish = [&](int tile, int buf, const RawRow<T, V, VEC>& x,
-                    const RawRow<T, V, VEC>& z) {
+  auto finish = [&](int tile, int buf, const RawRow<T, V, VEC>& x, const RawRow<T, V, VEC>& z) {
     const int t0 = tile * SSM_TT, rows = rows_of(tile);
     const rsrc_t ry = open_rsrc(yb);
-    {
-      float y[V];
+    float y[V] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-      for (int i = 0; i < V; ++i) y[i] = x.at(i) * D[i];
+    for (int j = 0; j < W; ++j) add_row(y, sy[STATE ? 0 : buf * W + j] + row * SSM_CH + tc);
 #pragma unroll
-      for (int j = 0; j < W; ++j) add_row(y, sy[STATE ? 0 : buf * W + j] + row * SSM_CH + tc);
-      RawRow<T, V, VEC> out;
+    for (int i = 0; i < V; ++i) y[i] = fmaf(x.at(i), D[i], y[i]);
+    if (has_z) {
+      if (p.mixed) {
+        RawRow<float, V, VEC> m;
+#pragma unroll
+        for (int i = 0; i < V; ++i) m.set(i, y[i]);
+        store_raw<float, V, VEC>(open_rsrc(p.mixed + ((long long)at.b * p.L + t0) * E + at.c0),
+                                 row * E + tc, row < rows, left, m);
+      }
 #pragma unroll
       for (int i = 0; i < V; ++i) {
         const float g = z.at(i);
-        if (has_z) y[i] *= g * sigmoid(g);
-        out.set(i, row < rows ? y[i] : 0.f);
+        y[i] *= g * sigmoid(g);
       }
-      store_raw<T, V, VEC>(ry, row * E + tc, row < p.L - t0, left, out);
     }
+    if (rows < SSM_TT && row >= rows) {
+#pragma unroll
+      for (int i = 0; i < V; ++i) y[i] = 0.f;
+    }
+    RawRow<T, V, VEC> out;
+#pragma unroll
+    for (int i = 0; i < V; ++i) out.set(i, y[i]);
+    store_raw<T, V, VEC>(ry, row * E + tc, row < p.L - t0, left, out);
     yb += SSM_TT * (long long)E;
   };
 
@@ -98,7 +110,7 @@ __global__ __launch_bounds__(64 * (W + SSM_HELPERS)) void ssm_fwd_kernel(Ssm p) 
   const T* Cb = (const T*)p.C + at.b * p.C_b + first * C_t + (long long)at.g * p.C_g;
   float* saved = p.saved ? p.saved + ((size_t)at.b * p.tiles + at.tile0) * N * E : nullptr;
   float A2[NP][4], h[NP][4], dsum = 0.f;
-  SsmVec<T> Bv[NP], Cv[NP];
+  SsmVec<T, 4> Bv[NP], Cv[NP];
   auto start = [&] {
 #pragma unroll
     for (int q = 0; q < NP; ++q)
@@ -174,7 +186,7 @@ __global__ __launch_bounds__(64 * (W + SSM_HELPERS)) void ssm_fwd_kernel(Ssm p) 
             hs[t][n] = h[q][n];
           });
         });
-        if (!STATE) ssm_dots(yl, Cf[q][i], hs);
+        if (!STATE) ssm_dots4(yl, Cf[q][i], hs);
       }
       if (!STATE) put_tokens(sy[STATE ? 0 : buf * W + w], 4 * i, lane, yl);
     }

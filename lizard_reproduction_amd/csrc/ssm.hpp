@@ -9,8 +9,8 @@ namespace lz {
 
 // Layout of the work.  A workgroup takes 64 channels of one group and one sequence (or a
 // segment of it) and walks it in tiles of 16 tokens.  In its W scan waves a lane is a
-// channel; wave w holds the states n = 4 w .. 4 w + 3 (and 4 (w + W) .. up to NP such),
-// four a lane, in registers.  Four helper waves turn the next tile's rows into delta, u and
+// channel; wave w holds NS states in registers, four in the forward (and another four from
+// 4 (w + W) on with NP = 2), two in the backward.  Four helper waves turn the next tile's rows into delta, u and
 // the like while the scan waves walk this one, and the last tile's sums into rows: one
 // barrier a tile, and waves to switch between though a wave holds 256 states.  (With the
 // scan waves doing both, two barriers a tile, the training pass of 8192 tokens x 4096
@@ -28,7 +28,8 @@ struct Ssm {
   float* state_out;
   const int* lengths;
   void* y;
-  float* saved;    // [B, tiles, N, E]: the state before each tile, for the backward
+  float* mixed;    // [B, L, E]: sum_n C h + D x, where z gates it, for the backward
+  float* saved;    // [B, tiles, N, E]: the state before each tile, likewise
   float* rec;      // [B, S - 1, N, E]: a segment's own state, from zero
   float* dsum;     // [B, S - 1, E]: its sum of delta
   long long x_b, dt_b, z_b, B_b, C_b, y_b;   // elements from one sequence to the next
@@ -47,7 +48,7 @@ struct SsmGrad {
   float* part_d;         // [B S, 2, E]: of dD and ddt_bias
   float* rec;            // as Ssm's, of the reverse walk
   float* dsum;
-  float* acc;            // [3][B, L, E]: sums over the states of earlier launches
+  float* acc;            // [2][B, L, E]: sums over the states of earlier launches
   long long acc_step;    // B L E
   int n0, first, last;   // this launch's first state; whether it is the first, the last
   int NQ;                // padded states in part_bc
@@ -88,18 +89,19 @@ __device__ __forceinline__ void put_tokens(float* tile, int t, int lane, const f
   for (int k = 0; k < 4; ++k) p[k * SSM_CH] = v[k];
 }
 
-// B or C of a tile for the four states of a wave: register i of a lane holds token
-// 4 i + (lane % 16) / 4, state lane % 4, so that token 4 i + k's state n is lane
-// 4 k + n of every row of 16, which a DPP operand broadcasts.
-template <typename T>
+// B or C of a tile for a wave's NS states (2 or 4): register i of a lane holds token
+// (16 / NS) i + (lane % 16) / NS, state lane % NS, so that the k-th token's state n of
+// register i is lane NS k + n of every row of 16, which a DPP operand broadcasts.
+template <typename T, int NS>
 struct SsmVec {
-  uint32_t w[4];
+  static constexpr int TOKENS = 16 / NS;   // a register
+  uint32_t w[NS];
   __device__ __forceinline__ void load(const T* base, int rows, int pitch, int N, int n0, int lane) {
     const rsrc_t r = open_rsrc(base);
-    const int n = n0 + (lane & 3);
+    const int n = n0 + lane % NS;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const int t = 4 * i + ((lane & 15) >> 2);
+    for (int i = 0; i < NS; ++i) {
+      const int t = TOKENS * i + lane % 16 / NS;
       const uint32_t at = t < rows && n < N ? (uint32_t)(t * pitch + n) * (uint32_t)sizeof(T) : OOB;
       if constexpr (IS_BF16<T>) w[i] = __builtin_amdgcn_raw_buffer_load_b16(r, at, 0, 0);
       else w[i] = __builtin_amdgcn_raw_buffer_load_b32(r, at, 0, 0);
@@ -110,38 +112,52 @@ struct SsmVec {
   }
 };
 
-// y[t] += sum_n v(4 t + n) h[t][n], v(k) lane k of a row of 16: the compiler folds the
-// broadcast into a product but not into a multiply-add, so these are written out, behind
-// the two wait states that a DPP operand asks for after its register was written.
-__device__ __forceinline__ void ssm_dots(f32x4& y, float v, const float (&h)[4][4]) {
-  float y0 = y[0], y1 = y[1], y2 = y[2], y3 = y[3];
+// y[t] += sum_n v(K + NS t + n) h[t][n] for four tokens t, v(k) lane k of a row of 16: the
+// compiler folds the broadcast into a product but not into a multiply-add, so these are
+// written out, behind the two wait states that a DPP operand asks for after its register
+// was written.
 #define LZ_DOT(t, k, n) \
+  "v_fmac_f32_dpp %" #t ", %4, %" #n " row_newbcast:%" #k " row_mask:0xf bank_mask:0xf\n"
+template <int K>
+__device__ __forceinline__ void ssm_dots(f32x4& y, float v, const float (&h)[4][2]) {
+  float y0 = y[0], y1 = y[1], y2 = y[2], y3 = y[3];
+  asm("s_nop 1\n"
+      LZ_DOT(0, 13, 5) LZ_DOT(1, 15, 7) LZ_DOT(2, 17, 9) LZ_DOT(3, 19, 11)
+      LZ_DOT(0, 14, 6) LZ_DOT(1, 16, 8) LZ_DOT(2, 18, 10) LZ_DOT(3, 20, 12)
+      : "+&v"(y0), "+&v"(y1), "+&v"(y2), "+&v"(y3)
+      : "v"(v), "v"(h[0][0]), "v"(h[0][1]), "v"(h[1][0]), "v"(h[1][1]), "v"(h[2][0]), "v"(h[2][1]),
+        "v"(h[3][0]), "v"(h[3][1]), "n"(K), "n"(K + 1), "n"(K + 2), "n"(K + 3), "n"(K + 4),
+        "n"(K + 5), "n"(K + 6), "n"(K + 7));
+  y = f32x4{y0, y1, y2, y3};
+}
+__device__ __forceinline__ void ssm_dots4(f32x4& y, float v, const float (&h)[4][4]) {
+  float y0 = y[0], y1 = y[1], y2 = y[2], y3 = y[3];
+#define LZ_DOT4(t, k, n) \
   "v_fmac_f32_dpp %" #t ", %4, %" #n " row_newbcast:" #k " row_mask:0xf bank_mask:0xf\n"
   asm("s_nop 1\n"
-      LZ_DOT(0, 0, 5) LZ_DOT(1, 4, 9) LZ_DOT(2, 8, 13) LZ_DOT(3, 12, 17)
-      LZ_DOT(0, 1, 6) LZ_DOT(1, 5, 10) LZ_DOT(2, 9, 14) LZ_DOT(3, 13, 18)
-      LZ_DOT(0, 2, 7) LZ_DOT(1, 6, 11) LZ_DOT(2, 10, 15) LZ_DOT(3, 14, 19)
-      LZ_DOT(0, 3, 8) LZ_DOT(1, 7, 12) LZ_DOT(2, 11, 16) LZ_DOT(3, 15, 20)
+      LZ_DOT4(0, 0, 5) LZ_DOT4(1, 4, 9) LZ_DOT4(2, 8, 13) LZ_DOT4(3, 12, 17)
+      LZ_DOT4(0, 1, 6) LZ_DOT4(1, 5, 10) LZ_DOT4(2, 9, 14) LZ_DOT4(3, 13, 18)
+      LZ_DOT4(0, 2, 7) LZ_DOT4(1, 6, 11) LZ_DOT4(2, 10, 15) LZ_DOT4(3, 14, 19)
+      LZ_DOT4(0, 3, 8) LZ_DOT4(1, 7, 12) LZ_DOT4(2, 11, 16) LZ_DOT4(3, 15, 20)
       : "+&v"(y0), "+&v"(y1), "+&v"(y2), "+&v"(y3)
       : "v"(v), "v"(h[0][0]), "v"(h[0][1]), "v"(h[0][2]), "v"(h[0][3]), "v"(h[1][0]),
         "v"(h[1][1]), "v"(h[1][2]), "v"(h[1][3]), "v"(h[2][0]), "v"(h[2][1]), "v"(h[2][2]),
         "v"(h[2][3]), "v"(h[3][0]), "v"(h[3][1]), "v"(h[3][2]), "v"(h[3][3]));
-#undef LZ_DOT
+#undef LZ_DOT4
   y = f32x4{y0, y1, y2, y3};
 }
+#undef LZ_DOT
 
-// g[n] = v(K + n) x + c[n], likewise
+// c[n] + v(K + n) x, likewise
 template <int K>
-__device__ __forceinline__ void ssm_fma4(float (&g)[4], float v, float x, const float (&c)[4]) {
-  float g0 = c[0], g1 = c[1], g2 = c[2], g3 = c[3];
+__device__ __forceinline__ void ssm_fma2(float (&g)[2], float v, float x, const float (&c)[2]) {
+  float g0 = c[0], g1 = c[1];
   asm("s_nop 1\n"
-      "v_fmac_f32_dpp %0, %4, %5 row_newbcast:%6 row_mask:0xf bank_mask:0xf\n"
-      "v_fmac_f32_dpp %1, %4, %5 row_newbcast:%7 row_mask:0xf bank_mask:0xf\n"
-      "v_fmac_f32_dpp %2, %4, %5 row_newbcast:%8 row_mask:0xf bank_mask:0xf\n"
-      "v_fmac_f32_dpp %3, %4, %5 row_newbcast:%9 row_mask:0xf bank_mask:0xf\n"
-      : "+&v"(g0), "+&v"(g1), "+&v"(g2), "+&v"(g3)
-      : "v"(v), "v"(x), "n"(K), "n"(K + 1), "n"(K + 2), "n"(K + 3));
-  g[0] = g0, g[1] = g1, g[2] = g2, g[3] = g3;
+      "v_fmac_f32_dpp %0, %2, %3 row_newbcast:%4 row_mask:0xf bank_mask:0xf\n"
+      "v_fmac_f32_dpp %1, %2, %3 row_newbcast:%5 row_mask:0xf bank_mask:0xf\n"
+      : "+&v"(g0), "+&v"(g1)
+      : "v"(v), "v"(x), "n"(K), "n"(K + 1));
+  g[0] = g0, g[1] = g1;
 }
 
 // Where a workgroup works
@@ -173,9 +189,11 @@ inline SsmWaves ssm_fwd_waves(int N) {
   return N <= 4 ? SsmWaves{1, 1} : N <= 8 ? SsmWaves{2, 1} : N <= 16 ? SsmWaves{4, 1}
        : N <= 32 ? SsmWaves{8, 1} : SsmWaves{8, 2};
 }
-// States the backward takes a launch, and N in whole waves
+// States the backward takes a launch, and N padded to whole launches
 constexpr int SSM_BWD_STATES = 16;
-inline int ssm_bwd_padded(int N) { return (N + 3) / 4 * 4 <= 4 ? 4 : N <= 8 ? 8 : (N + 15) / 16 * 16; }
+inline int ssm_bwd_padded(int N) {
+  return N <= 2 ? 2 : N <= 4 ? 4 : N <= 8 ? 8 : (N + 15) / 16 * 16;
+}
 
 int ssm_segments(int batch, int G, int Eg, int L, bool backward);
 hipError_t launch_ssm_fwd(const Ssm& p, bool is_bf16, bool vec, hipStream_t st);

@@ -9,18 +9,18 @@
 //
 // The forward kept the state before each tile of 16 tokens.  A workgroup takes 64 channels
 // as in the forward and walks the tiles from the last; in each it walks forward once, every
-// decay and state of its 16 tokens staying in registers (128 of them), then back.  What is
+// decay and state of its 16 tokens staying in registers, then back.  What is
 // summed over n meets in LDS, the waves' shares side by side; what is summed over channels
-// is added across the wave, eight sums at a time, each step halving the lanes that carry
-// one (17 instructions for the 8 sums of 64 lanes), and its 64-channel shares, as the
-// sequences' shares of dA, dD and dbias, go to memory for a second launch that adds them in
+// is added across the wave, two tokens' eight sums at a time, and its 64-channel shares, as the sequences' shares
+// of dA, dD and dbias, go to memory for a second launch that adds them in
 // order: no atomics, the same bits every time.  More than 16 states are taken 16 a launch
 // (in one, a wave's registers did not hold them: N = 24 took 2.8 times as long as 16).
 #include "ssm.hpp"
 
 namespace lz {
 
-// The sums of v0 .. v7 over the wave: lane l gets sum l / 8.
+// The sums of v0 .. v7 over the wave, each step halving the registers that carry them:
+// lane l gets sum l / 8.
 __device__ __forceinline__ float wave_sums8(const float (&v)[8]) {
   float q[4], r[2];
 #pragma unroll
@@ -41,20 +41,19 @@ __device__ __forceinline__ float wave_sums8(const float (&v)[8]) {
 // segments but the first.
 template <int W, bool STATE>
 constexpr int ssm_bwd_lds() {   // tiles, two of each
-  return 2 * (STATE ? 2 : 3 + 3 * W);
+  return 2 * (STATE ? 2 : 3 + 2 * W);
 }
 
 template <typename T, int W, bool VEC, bool STATE>
-__global__ __launch_bounds__(64 * (W + SSM_HELPERS), 2) void ssm_bwd_kernel(Ssm p, SsmGrad gr) {
+__global__ __launch_bounds__(64 * (W + SSM_HELPERS), W == 8 ? 3 : 2) void ssm_bwd_kernel(Ssm p, SsmGrad gr) {
   constexpr int V = SSM_V;
   extern __shared__ float lds[];
   auto sd = [&](int buf) { return lds + buf * SSM_TILE; };              // delta
   auto sg = [&](int buf) { return lds + (2 + buf) * SSM_TILE; };      // dm
   auto su = [&](int buf) { return lds + (4 + buf) * SSM_TILE; };  // delta x
-  // the waves' shares of du, of sum_n v A and of sum_n C h
+  // the waves' shares of du and of sum_n v A
   auto pu = [&](int buf, int j) { return lds + ((3 + j) * 2 + buf) * SSM_TILE; };
   auto pd = [&](int buf, int j) { return lds + ((3 + W + j) * 2 + buf) * SSM_TILE; };
-  auto py = [&](int buf, int j) { return lds + ((3 + 2 * W + j) * 2 + buf) * SSM_TILE; };
   const int segments = STATE ? p.S - 1 : p.S;
   SsmPlace at(p, segments);
   if constexpr (STATE) {   // segments 1 .. S - 1
@@ -78,9 +77,12 @@ __global__ __launch_bounds__(64 * (W + SSM_HELPERS), 2) void ssm_bwd_kernel(Ssm 
   const T* db = (const T*)p.dt + at.b * p.dt_b + last * dt_t + at.c0;
   const T* zb = has_z ? (const T*)p.z + at.b * p.z_b + last * z_t + at.c0 : nullptr;
   const T* dyb = (const T*)gr.dy + ((long long)at.b * p.L + last) * E + at.c0;
-  struct Rows {
-    RawRow<T, V, VEC> x, dt, z, dy;
-  } next;
+  const float* mb = p.mixed + ((long long)at.b * p.L + last) * E + at.c0;
+  RawRow<T, V, VEC> xr, dr, zr, yr;   // the next tile's rows
+  RawRow<float, V, VEC> mr;
+  struct Kept {                       // of a tile, from its beginning to its end
+    float x[V], dm[V], slope[V], dz[V];
+  };
   auto load_params = [&] {
 #pragma unroll
     for (int i = 0; i < V; ++i) {
@@ -91,62 +93,78 @@ __global__ __launch_bounds__(64 * (W + SSM_HELPERS), 2) void ssm_bwd_kernel(Ssm 
   };
   auto load_rows = [&](int rows) {
     const rsrc_t rx = open_rsrc(xb), rd = open_rsrc(db), rz = open_rsrc(zb), ry = open_rsrc(dyb);
-    {
-      if (!STATE) next.x = load_raw<T, V, VEC>(rx, row * x_t + tc, row < rows, left);
-      next.dt = load_raw<T, V, VEC>(rd, row * dt_t + tc, row < rows, left);
-      next.z = load_raw<T, V, VEC>(rz, row * z_t + tc, has_z && row < rows, left);
-      next.dy = load_raw<T, V, VEC>(ry, row * E + tc, row < rows, left);
+    if (!STATE) xr = load_raw<T, V, VEC>(rx, row * x_t + tc, row < rows, left);
+    dr = load_raw<T, V, VEC>(rd, row * dt_t + tc, row < rows, left);
+    zr = load_raw<T, V, VEC>(rz, row * z_t + tc, has_z && row < rows, left);
+    yr = load_raw<T, V, VEC>(ry, row * E + tc, row < rows, left);
+    if (!STATE) {
+      mr = load_raw<float, V, VEC>(open_rsrc(mb), row * E + tc, has_z && row < rows, left);
+      mb -= SSM_TT * (long long)E;
     }
     xb -= SSM_TT * (long long)x_t;
     db -= SSM_TT * (long long)dt_t;
     if (has_z) zb -= SSM_TT * (long long)z_t;
     dyb -= SSM_TT * (long long)E;
   };
-  auto prep = [&](int rows, int buf) {
-    {
-      const int e = row * SSM_CH + tc;
-      float d[V], u[V], dm[V];
+  auto prep = [&](int rows, int buf, Kept& k) {
+    const int e = row * SSM_CH + tc;
+    float d[V], u[V];
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+      const float pre = dr.at(i) + bias[i];
+      d[i] = pre, k.slope[i] = 1.f;
+      if (soft) d[i] = STATE ? softplus(pre) : softplus_slope(pre, k.slope[i]);
+      k.dm[i] = yr.at(i);
+      if (!STATE) k.x[i] = xr.at(i);
+    }
+    if (has_z) {
 #pragma unroll
       for (int i = 0; i < V; ++i) {
-        const float pre = next.dt.at(i) + bias[i], z = next.z.at(i), dy = next.dy.at(i);
-        d[i] = row < rows ? soft ? softplus(pre) : pre : 0.f;
-        dm[i] = has_z ? dy * (z * sigmoid(z)) : dy;
-        if (!STATE) u[i] = d[i] * next.x.at(i);
+        const float z = zr.at(i), s = sigmoid(z), dy = k.dm[i], zs = z * s;
+        k.dm[i] = dy * zs;
+        if (!STATE) k.dz[i] = dy * mr.at(i) * fmaf(zs, 1.f - s, s);
       }
-      put_row(sd(buf) + e, d);
-      put_row(sg(buf) + e, dm);
-      if (!STATE) put_row(su(buf) + e, u);
+    }
+    if (rows < SSM_TT && row >= rows) {
+#pragma unroll
+      for (int i = 0; i < V; ++i) d[i] = 0.f;
+    }
+    put_row(sd(buf) + e, d);
+    put_row(sg(buf) + e, k.dm);
+    if (!STATE) {
+#pragma unroll
+      for (int i = 0; i < V; ++i) u[i] = d[i] * k.x[i];
+      put_row(su(buf) + e, u);
     }
   };
-  auto finish = [&](int tile, int buf, const Rows& now) {
+  auto finish = [&](int tile, int buf, const Kept& k) {
     const int rows = rows_of(tile), e = row * SSM_CH + tc;
     const long long o = ((long long)at.b * p.L + (long long)tile * SSM_TT) * E + at.c0;
     const uint32_t off = row * E + tc;
     const bool in = row < rows;
-    float sum[3][V];   // of du, of sum_n v A and of sum_n C h
+    float sum[2][V];   // of du and of sum_n v A
 #pragma unroll
-    for (int i = 0; i < V; ++i) sum[0][i] = sum[1][i] = 0.f, sum[2][i] = now.x.at(i) * D[i];
+    for (int i = 0; i < V; ++i) sum[0][i] = sum[1][i] = 0.f;
     if (!gr.first) {
 #pragma unroll
-      for (int k = 0; k < 3; ++k) {
-        const auto r = load_raw<float, V, VEC>(open_rsrc(gr.acc + k * gr.acc_step + o), off, in, left);
+      for (int j = 0; j < 2; ++j) {
+        const auto r = load_raw<float, V, VEC>(open_rsrc(gr.acc + j * gr.acc_step + o), off, in, left);
 #pragma unroll
-        for (int i = 0; i < V; ++i) sum[k][i] = r.at(i);
+        for (int i = 0; i < V; ++i) sum[j][i] = r.at(i);
       }
     }
 #pragma unroll
     for (int j = 0; j < W; ++j) {
       add_row(sum[0], pu(buf, j) + e);
       add_row(sum[1], pd(buf, j) + e);
-      if (has_z) add_row(sum[2], py(buf, j) + e);
     }
     if (!gr.last) {
 #pragma unroll
-      for (int k = 0; k < 3; ++k) {
+      for (int j = 0; j < 2; ++j) {
         RawRow<float, V, VEC> r;
 #pragma unroll
-        for (int i = 0; i < V; ++i) r.set(i, sum[k][i]);
-        store_raw<float, V, VEC>(open_rsrc(gr.acc + k * gr.acc_step + o), off, in, left, r);
+        for (int i = 0; i < V; ++i) r.set(i, sum[j][i]);
+        store_raw<float, V, VEC>(open_rsrc(gr.acc + j * gr.acc_step + o), off, in, left, r);
       }
       return;
     }
@@ -155,20 +173,12 @@ __global__ __launch_bounds__(64 * (W + SSM_HELPERS), 2) void ssm_bwd_kernel(Ssm 
     add_row(d, sd(buf) + e);
 #pragma unroll
     for (int i = 0; i < V; ++i) {
-      const float x = now.x.at(i), dy = now.dy.at(i);
-      float dm = dy, ddt = fmaf(x, sum[0][i], sum[1][i] * LN2);
-      if (has_z) {
-        const float z = now.z.at(i), sz = sigmoid(z);
-        dm = dy * (z * sz);
-        oz.set(i, dy * sum[2][i] * (sz * fmaf(z, 1.f - sz, 1.f)));
-      }
-      if (soft) ddt *= sigmoid(now.dt.at(i) + bias[i]);
-      ox.set(i, fmaf(d[i], sum[0][i], D[i] * dm));
+      const float ddt = fmaf(k.x[i], sum[0][i], sum[1][i] * LN2) * k.slope[i];
+      ox.set(i, fmaf(d[i], sum[0][i], D[i] * k.dm[i]));
       od.set(i, ddt);
-      if (in && i < left) {
-        dD[i] += dm * x;
-        dbias[i] += ddt;
-      }
+      if (has_z) oz.set(i, k.dz[i]);
+      dD[i] = fmaf(k.dm[i], k.x[i], dD[i]);   // x and dy are zero where there is no row
+      if (in && i < left) dbias[i] += ddt;
     }
     store_raw<T, V, VEC>(open_rsrc((T*)gr.dx + o), off, in, left, ox);
     store_raw<T, V, VEC>(open_rsrc((T*)gr.ddt + o), off, in, left, od);
@@ -176,7 +186,7 @@ __global__ __launch_bounds__(64 * (W + SSM_HELPERS), 2) void ssm_bwd_kernel(Ssm 
   };
 
   // --- the walk (scan) --------------------------------------------------------------------
-  const int w = wave, c = at.c0 + lane, n0 = gr.n0 + 4 * w;
+  const int w = wave, c = at.c0 + lane, n0 = gr.n0 + 2 * w;
   const bool mine = lane < at.cols;
   const int B_t = p.B_t, C_t = p.C_t;
   const T* Bb = (const T*)p.B + at.b * p.B_b + last * B_t + (long long)at.g * p.B_g;
@@ -185,12 +195,12 @@ __global__ __launch_bounds__(64 * (W + SSM_HELPERS), 2) void ssm_bwd_kernel(Ssm 
   float* bc = STATE ? nullptr
                     : gr.part_bc + (((long long)at.blk * p.batch + at.b) * p.L + last) * 2 * gr.NQ;
   const int NQ = gr.NQ;
-  float A2[4], carry[4], dA[4], dsum = 0.f;
-  SsmVec<T> Bv, Cv;
-  float h0[4];
+  float A2[2], carry[2], dA[2], dsum = 0.f;
+  SsmVec<T, 2> Bv, Cv;
+  float h0[2];
   auto start = [&] {
 #pragma unroll
-      for (int k = 0; k < 4; ++k) {
+      for (int k = 0; k < 2; ++k) {
         const int n = n0 + k;
         A2[k] = mine && n < N ? p.A[(size_t)c * N + n] * LOG2E : 0.f;
         carry[k] = dA[k] = 0.f;
@@ -215,7 +225,7 @@ __global__ __launch_bounds__(64 * (W + SSM_HELPERS), 2) void ssm_bwd_kernel(Ssm 
     Cv.load(Cb, rows, C_t, N, n0, lane);
     if (!STATE) {
 #pragma unroll
-      for (int k = 0; k < 4; ++k) {
+      for (int k = 0; k < 2; ++k) {
         const int n = n0 + k;
         h0[k] = mine && n < N ? saved[(size_t)n * E] : 0.f;
       }
@@ -227,89 +237,71 @@ __global__ __launch_bounds__(64 * (W + SSM_HELPERS), 2) void ssm_bwd_kernel(Ssm 
     saved -= (size_t)N * E;
   };
   auto scan_state = [&](int buf) {
-    float Cf[4];
-#pragma unroll
-    for (int i = 0; i < 4; ++i) Cf[i] = Cv.at(i);
-#pragma unroll
-    for (int i = 3; i >= 0; --i) {
+    const float Cf[2] = {Cv.at(0), Cv.at(1)};
+    static_for<4>([&](auto ki) {
+      constexpr int i = 3 - decltype(ki)::value;
       const f32x4 d4 = get_tokens(sd(buf), 4 * i, lane), g4 = get_tokens(sg(buf), 4 * i, lane);
       dsum += (d4[0] + d4[1]) + (d4[2] + d4[3]);
       static_for<4>([&](auto kt) {
         constexpr int t = 3 - decltype(kt)::value;
-        float g[4];
-        ssm_fma4<4 * t>(g, Cf[i], g4[t], carry);
+        float g[2];
+        ssm_fma2<8 * (i & 1) + 2 * t>(g, Cf[i >> 1], g4[t], carry);
 #pragma unroll
-        for (int n = 0; n < 4; ++n) carry[n] = __builtin_amdgcn_exp2f(d4[t] * A2[n]) * g[n];
+        for (int n = 0; n < 2; ++n) carry[n] = __builtin_amdgcn_exp2f(d4[t] * A2[n]) * g[n];
       });
-    }
+    });
   };
   auto scan = [&](int tile, int buf, bool more) {
     const int rows = rows_of(tile);
-    float a[16][4], h[16][4], Bf[4], Cf[4], hb[4], bcsum[2] = {0.f, 0.f};
-#pragma unroll
-    for (int i = 0; i < 4; ++i) Bf[i] = Bv.at(i), Cf[i] = Cv.at(i), hb[i] = h0[i];
+    const float Bf[2] = {Bv.at(0), Bv.at(1)}, Cf[2] = {Cv.at(0), Cv.at(1)}, hb[2] = {h0[0], h0[1]};
+    float a[16][2], h[16][2], bcsum = 0.f, v8[8];
     if (more) load_bc(SSM_TT);
     // forward over the tile
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const f32x4 d4 = get_tokens(sd(buf), 4 * i, lane), u4 = get_tokens(su(buf), 4 * i, lane);
-      float hs[4][4];
-      static_for<4>([&](auto kt) {
-        constexpr int t = decltype(kt)::value;
-        static_for<4>([&](auto kn) {
-          constexpr int n = decltype(kn)::value;
-          const float before = 4 * i + t ? h[(4 * i + t + 15) % 16][n] : hb[n];
-          a[4 * i + t][n] = __builtin_amdgcn_exp2f(d4[t] * A2[n]);
-          h[4 * i + t][n] = fmaf(a[4 * i + t][n], before,
-                                 dpp<DPP_BCAST + 4 * t + n>(Bf[i]) * u4[t]);
-          hs[t][n] = h[4 * i + t][n];
-        });
+    static_for<16>([&](auto kt) {
+      constexpr int tt = decltype(kt)::value;
+      const float d = sd(buf)[tt * SSM_CH + lane], u = su(buf)[tt * SSM_CH + lane];
+      static_for<2>([&](auto kn) {
+        constexpr int n = decltype(kn)::value;
+        a[tt][n] = __builtin_amdgcn_exp2f(d * A2[n]);
+        h[tt][n] = fmaf(a[tt][n], tt ? h[(tt + 15) % 16][n] : hb[n],
+                        dpp<DPP_BCAST + 2 * (tt & 7) + n>(Bf[tt >> 3]) * u);
       });
-      if (has_z) {
-        f32x4 yl = {0.f, 0.f, 0.f, 0.f};
-        ssm_dots(yl, Cf[i], hs);
-        put_tokens(py(buf, w), 4 * i, lane, yl);
-      }
-    }
+    });
     // and back
-#pragma unroll
-    for (int i = 3; i >= 0; --i) {
+    static_for<4>([&](auto ki) {
+      constexpr int i = 3 - decltype(ki)::value, K = 8 * (i & 1);
       const f32x4 d4 = get_tokens(sd(buf), 4 * i, lane), u4 = get_tokens(su(buf), 4 * i, lane);
       const f32x4 g4 = get_tokens(sg(buf), 4 * i, lane);
-      float gs[4][4];
+      float gs[4][2];
       f32x4 dv = {0.f, 0.f, 0.f, 0.f}, du = {0.f, 0.f, 0.f, 0.f};
       static_for<4>([&](auto kt) {
-        constexpr int t = 3 - decltype(kt)::value;
-        const int tt = 4 * i + t;
-        float v8[8];
-        ssm_fma4<4 * t>(gs[t], Cf[i], g4[t], carry);
-        static_for<4>([&](auto kn) {
-          constexpr int n = decltype(kn)::value;
+        constexpr int t = 3 - decltype(kt)::value, tt = 4 * i + t, to = tt & 1 ? 0 : 4;
+        ssm_fma2<K + 2 * t>(gs[t], Cf[i >> 1], g4[t], carry);
+#pragma unroll
+        for (int n = 0; n < 2; ++n) {
           const float g = gs[t][n];
-          v8[n] = g * u4[t];
-          v8[4 + n] = g4[t] * h[tt][n];
+          v8[to + n] = g * u4[t];
+          v8[to + 2 + n] = g4[t] * h[tt][n];
           carry[n] = a[tt][n] * g;
           const float v = carry[n] * (tt ? h[(tt + 15) % 16][n] : hb[n]);
           dv[t] = fmaf(v, A2[n], dv[t]);
           dA[n] = fmaf(v, d4[t], dA[n]);
-        });
-        const float s8 = wave_sums8(v8);
-        if ((lane & 7) == (tt & 7)) bcsum[tt >> 3] = s8;
+        }
+        if (tt % 2 == 0) {   // tokens tt + 1 and tt
+          const float s = wave_sums8(v8);
+          if ((lane & 7) == tt / 2) bcsum = s;
+        }
       });
-      ssm_dots(du, Bf[i], gs);
+      ssm_dots<K>(du, Bf[i >> 1], gs);
       put_tokens(pd(buf, w), 4 * i, lane, dv);
       put_tokens(pu(buf, w), 4 * i, lane, du);
-    }
-    // lane l: of token l % 8 (+ 8), B's (l < 32) or C's sum for state (l / 8) % 4
-    const rsrc_t rb = open_rsrc(bc);
-#pragma unroll
-    for (int k = 0; k < 2; ++k) {
-      const int row = 8 * k + (lane & 7), idx = lane >> 3;
-      const uint32_t off =
-          (uint32_t)((2 * row + (idx >> 2)) * NQ + n0 + (idx & 3)) * 4u;
-      __builtin_amdgcn_raw_buffer_store_b32(__builtin_bit_cast(uint32_t, bcsum[k]), rb,
-                                            row < rows ? off : OOB, 0, 0);
-    }
+    });
+    // lane l: of token 2 (l % 8) + 1 (l < 32) or 2 (l % 8), B's or C's (l / 16 % 2), state
+    // l / 8 % 2
+    const int tk = 2 * (lane & 7) + (lane < 32);
+    const uint32_t off = (uint32_t)((2 * tk + (lane >> 4 & 1)) * NQ + n0 + (lane >> 3 & 1)) * 4u;
+    __builtin_amdgcn_raw_buffer_store_b32(__builtin_bit_cast(uint32_t, bcsum), open_rsrc(bc),
+                                          tk < rows ? off : OOB, 0, 0);
     bc -= SSM_TT * 2 * NQ;
   };
   auto end = [&] {
@@ -317,7 +309,7 @@ __global__ __launch_bounds__(64 * (W + SSM_HELPERS), 2) void ssm_bwd_kernel(Ssm 
     const size_t rec = (size_t)at.b * (p.S - 1) + at.s - 1, part = (size_t)at.b * p.S + at.s;
     if (STATE && w == 0) gr.dsum[rec * E + c] = dsum;
 #pragma unroll
-    for (int k = 0; k < 4; ++k) {
+    for (int k = 0; k < 2; ++k) {
       const int n = n0 + k;
       if (n >= N) continue;
       if (STATE) gr.rec[(rec * N + n) * E + c] = carry[k];
@@ -327,11 +319,10 @@ __global__ __launch_bounds__(64 * (W + SSM_HELPERS), 2) void ssm_bwd_kernel(Ssm 
 
   const int t0 = at.tile0, t1 = at.tile1;   // t0 < t1
   if (wave >= W) {
-    Rows now, before;   // of this tile and the one after it in the sequence
+    Kept now, before;   // of this tile and the one after it in the sequence
     load_params();
     load_rows(rows_of(t1 - 1));
-    prep(rows_of(t1 - 1), 0);
-    now = next;
+    prep(rows_of(t1 - 1), 0, now);
     if (t1 - 1 > t0) load_rows(SSM_TT);
     __syncthreads();
     for (int tile = t1 - 1; tile >= t0; --tile) {
@@ -339,8 +330,7 @@ __global__ __launch_bounds__(64 * (W + SSM_HELPERS), 2) void ssm_bwd_kernel(Ssm 
       if (!STATE && tile < t1 - 1) finish(tile + 1, buf ^ 1, before);
       before = now;
       if (tile > t0) {
-        prep(SSM_TT, buf ^ 1);
-        now = next;
+        prep(SSM_TT, buf ^ 1, now);
         if (tile - 1 > t0) load_rows(SSM_TT);
       }
       __syncthreads();
@@ -410,9 +400,10 @@ hipError_t bwd_waves(const Ssm& p, SsmGrad gr, hipStream_t st) {
     const int n = p.N - gr.n0;
     gr.first = gr.n0 == 0;
     gr.last = n <= SSM_BWD_STATES;
-    const hipError_t e = n <= 4   ? bwd_launch<T, 1, VEC>(p, gr, st)
-                         : n <= 8 ? bwd_launch<T, 2, VEC>(p, gr, st)
-                                  : bwd_launch<T, 4, VEC>(p, gr, st);
+    const hipError_t e = n <= 2   ? bwd_launch<T, 1, VEC>(p, gr, st)
+                         : n <= 4 ? bwd_launch<T, 2, VEC>(p, gr, st)
+                         : n <= 8 ? bwd_launch<T, 4, VEC>(p, gr, st)
+                                  : bwd_launch<T, 8, VEC>(p, gr, st);
     if (e != hipSuccess) return e;
   }
   return hipSuccess;

@@ -767,7 +767,8 @@ def ssm(x, dt, A, B, C, D=None, z=None, dt_bias=None, dt_softplus=True):
     x, dt, z ``[B, L, E]``; A ``[E, N]`` (N at most 64), D, dt_bias ``[E]``; B, C
     ``[B, L, N]``, or ``[B, L, G, N]`` with E / G consecutive channels to each of
     the G.  Returns y ``[B, L, E]``.  The backward reads states that the
-    forward keeps, one every 16 tokens (N / 4 bytes a token and channel)."""
+    forward keeps, one every 16 tokens (N / 4 bytes a token and channel), and with z
+    the rows that it gates (4 bytes)."""
     B, C = _check_ssm("ssm", x, dt, A, B, C, D, z, dt_bias, False)
     return _ops.load().ssm(x, dt, A, B, C, D, z, dt_bias, bool(dt_softplus))
 

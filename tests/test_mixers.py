@@ -325,8 +325,9 @@ def test_norm_entry_points_refuse(lib):  # noqa: F811
 
 def test_workspaces_of_refused_sizes_are_empty(lib):  # noqa: F811
     assert lib.lz_ssm_bwd_workspace_bytes(1, 16, 8, 65, 1) == 0
-    assert lib.lz_ssm_states_bytes(0, 16, 8, 4) == 0
-    assert lib.lz_ssm_states_bytes(2, 17, 8, 4) == 2 * 2 * 8 * 4 * 4
+    assert lib.lz_ssm_states_bytes(0, 16, 8, 4, 1) == 0
+    assert lib.lz_ssm_states_bytes(2, 17, 8, 4, 0) == 2 * 2 * 8 * 4 * 4
+    assert lib.lz_ssm_states_bytes(2, 17, 8, 4, 1) == 2 * (2 * 4 + 17) * 8 * 4
     assert lib.lz_group_norm_bwd_workspace_bytes(1, 1, 1, 8193) == 0
     # sequences and channels that fill the GPU by themselves are not split
     assert lib.lz_ssm_fwd_workspace_bytes(64, 2048, 4096, 16, 1) == 0
