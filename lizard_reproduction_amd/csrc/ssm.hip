@@ -12,9 +12,9 @@
 namespace lz {
 
 // STATE: the segments' own states alone, without C, z and y.
-template <typename T, int W, int NP, bool VEC, bool STATE>
-__global__ __launch_bounds__(64 * (W + SSM_HELPERS)) void ssm_fwd_kernel(Ssm p) {
-  constexpr int V = SSM_V;
+template <typename T, int W, int NP, int H, bool VEC, bool STATE>
+__global__ __launch_bounds__(64 * (W + H)) void ssm_fwd_kernel(Ssm p) {
+  constexpr int V = SSM_TILE / (64 * H), COLS = SSM_CH / V;
   // two tiles of each: one worked on by the scan waves, one by the helpers
   __shared__ float sd[2][SSM_TILE], su[2][SSM_TILE], sy[STATE ? 1 : 2 * W][SSM_TILE];
   const int segments = STATE ? p.S - 1 : p.S;
@@ -27,14 +27,16 @@ __global__ __launch_bounds__(64 * (W + SSM_HELPERS)) void ssm_fwd_kernel(Ssm p) 
 
   // --- rows to delta and u, shares of y to rows (helper) ------------------------------
   const int tid = (int)threadIdx.x - 64 * W;
-  const int row = tid / SSM_COLS, tc = (tid % SSM_COLS) * V, left = at.cols - tc;
+  const int row = tid / COLS, tc = (tid % COLS) * V, left = at.cols - tc;
   const bool has_z = p.z, soft = p.softplus;
   const int x_t = p.x_t, dt_t = p.dt_t, z_t = p.z_t;
   const T* xb = (const T*)p.x + at.b * p.x_b + first * x_t + at.c0;
   const T* db = (const T*)p.dt + at.b * p.dt_b + first * dt_t + at.c0;
   const T* zb = has_z ? (const T*)p.z + at.b * p.z_b + first * z_t + at.c0 : nullptr;
   T* yb = (T*)p.y + ((long long)at.b * p.L + first) * E + at.c0;
-  RawRow<T, V, VEC> xr, dr, zr;   // the next tile's rows
+  struct Rows {   // of a tile
+    RawRow<T, V, VEC> x, dt, z;
+  };
   float bias[V], D[V];
   auto load_params = [&] {
 #pragma unroll
@@ -43,24 +45,21 @@ __global__ __launch_bounds__(64 * (W + SSM_HELPERS)) void ssm_fwd_kernel(Ssm p) 
       D[i] = !STATE && p.D && i < left ? p.D[at.c0 + tc + i] : 0.f;
     }
   };
-  auto load_rows = [&](int rows) {
-    const rsrc_t rx = open_rsrc(xb), rd = open_rsrc(db), rz = open_rsrc(zb);
-    {
-      xr = load_raw<T, V, VEC>(rx, row * x_t + tc, row < rows, left);
-      dr = load_raw<T, V, VEC>(rd, row * dt_t + tc, row < rows, left);
-      if (!STATE) zr = load_raw<T, V, VEC>(rz, row * z_t + tc, has_z && row < rows, left);
-    }
+  auto load_rows = [&](int rows, Rows& r) {
+    r.x = load_raw<T, V, VEC>(open_rsrc(xb), row * x_t + tc, row < rows, left);
+    r.dt = load_raw<T, V, VEC>(open_rsrc(db), row * dt_t + tc, row < rows, left);
+    if (!STATE) r.z = load_raw<T, V, VEC>(open_rsrc(zb), row * z_t + tc, has_z && row < rows, left);
     xb += SSM_TT * (long long)x_t;
     db += SSM_TT * (long long)dt_t;
     if (has_z) zb += SSM_TT * (long long)z_t;
   };
-  auto prep = [&](int rows, int buf) {
+  auto prep = [&](int rows, int buf, const Rows& r) {
     float d[V], u[V];
 #pragma unroll
     for (int i = 0; i < V; ++i) {
-      d[i] = dr.at(i) + bias[i];
+      d[i] = r.dt.at(i) + bias[i];
       if (soft) d[i] = softplus(d[i]);
-      u[i] = d[i] * xr.at(i);
+      u[i] = d[i] * r.x.at(i);
     }
     if (rows < SSM_TT && row >= rows) {   // past the length: the state stays as it is
 #pragma unroll
@@ -72,7 +71,7 @@ __global__ __launch_bounds__(64 * (W + SSM_HELPERS)) void ssm_fwd_kernel(Ssm p) 
   auto finish = [&](int tile, int buf, const RawRow<T, V, VEC>& x, const RawRow<T, V, VEC>& z) {
     const int t0 = tile * SSM_TT, rows = rows_of(tile);
     const rsrc_t ry = open_rsrc(yb);
-    float y[V] = {0.f, 0.f, 0.f, 0.f};
+    float y[V] = {};
 #pragma unroll
     for (int j = 0; j < W; ++j) add_row(y, sy[STATE ? 0 : buf * W + j] + row * SSM_CH + tc);
 #pragma unroll
@@ -210,25 +209,33 @@ __global__ __launch_bounds__(64 * (W + SSM_HELPERS)) void ssm_fwd_kernel(Ssm p) 
 
   const int t0 = at.tile0, t1 = at.tile1;   // t0 < t1
   if (wave >= W) {
-    RawRow<T, V, VEC> x1, z1, x0, z0;   // of this tile and the one before
+    // the rows of two tiles ahead on their way, of this tile and the one before kept to
+    // their end; a tile's sums go out after the next rows have come, so that nothing waits
+    // for a store
+    Rows even, odd, now, last, before;
     load_params();
-    load_rows(rows_of(t0));
-    prep(rows_of(t0), 0);
-    x1 = xr, z1 = zr;
-    if (t0 + 1 < t1) load_rows(rows_of(t0 + 1));
+    load_rows(rows_of(t0), even);
+    if (t0 + 1 < t1) load_rows(rows_of(t0 + 1), odd);
+    prep(rows_of(t0), 0, even);
+    now = even;
+    if (t0 + 2 < t1) load_rows(rows_of(t0 + 2), even);
     __syncthreads();
-    for (int tile = t0; tile < t1; ++tile) {
-      const int buf = (tile - t0) & 1;
-      if (!STATE && tile > t0) finish(tile - 1, buf ^ 1, x0, z0);
-      x0 = x1, z0 = z1;
+    auto step = [&](int tile, int buf, Rows& next) {
+      before = now;
       if (tile + 1 < t1) {
-        prep(rows_of(tile + 1), buf ^ 1);
-        x1 = xr, z1 = zr;
-        if (tile + 2 < t1) load_rows(rows_of(tile + 2));
+        prep(rows_of(tile + 1), buf ^ 1, next);
+        now = next;
+        if (tile + 3 < t1) load_rows(rows_of(tile + 3), next);
       }
+      if (!STATE && tile > t0) finish(tile - 1, buf ^ 1, last.x, last.z);
+      last = before;
       __syncthreads();
+    };
+    for (int tile = t0; tile < t1; tile += 2) {
+      step(tile, 0, odd);
+      if (tile + 1 < t1) step(tile + 1, 1, even);
     }
-    if (!STATE) finish(t1 - 1, (t1 - 1 - t0) & 1, x0, z0);
+    if (!STATE) finish(t1 - 1, (t1 - 1 - t0) & 1, last.x, last.z);
   } else {
     load_bc(rows_of(t0));
     start();
@@ -304,16 +311,20 @@ __global__ __launch_bounds__(256) void ssm_step_kernel(Ssm p, float* state) {
   }
 }
 
+#ifndef HELPERS
+#define HELPERS 8
+#endif
 template <typename T, int W, int NP, bool VEC>
 hipError_t fwd_launch(const Ssm& p, hipStream_t st) {
   const int nblk = p.G * p.gblocks;
-  const dim3 block(64 * (W + SSM_HELPERS));
+  constexpr int H = HELPERS;
+  const dim3 block(64 * (W + H));
   if (p.S > 1) {
-    hipLaunchKernelGGL((ssm_fwd_kernel<T, W, NP, VEC, true>), dim3(nblk * (p.S - 1) * p.batch),
+    hipLaunchKernelGGL((ssm_fwd_kernel<T, W, NP, H, VEC, true>), dim3(nblk * (p.S - 1) * p.batch),
                        block, 0, st, p);
     if (hipError_t e = hipGetLastError(); e != hipSuccess) return e;
   }
-  hipLaunchKernelGGL((ssm_fwd_kernel<T, W, NP, VEC, false>), dim3(nblk * p.S * p.batch), block,
+  hipLaunchKernelGGL((ssm_fwd_kernel<T, W, NP, H, VEC, false>), dim3(nblk * p.S * p.batch), block,
                      0, st, p);
   return hipGetLastError();
 }

@@ -70,13 +70,20 @@ __device__ __forceinline__ void static_for(F f) {
 }
 
 // A thread's vector of a tile
-__device__ __forceinline__ void put_row(float* to, const float (&v)[SSM_V]) {
-  *reinterpret_cast<f32x4*>(to) = f32x4{v[0], v[1], v[2], v[3]};
-}
-__device__ __forceinline__ void add_row(float (&v)[SSM_V], const float* from) {
-  const f32x4 x = *reinterpret_cast<const f32x4*>(from);
+template <int V>
+__device__ __forceinline__ void put_row(float* to, const float (&v)[V]) {
+  typedef float vec __attribute__((ext_vector_type(V)));
+  vec x;
 #pragma unroll
-  for (int k = 0; k < SSM_V; ++k) v[k] += x[k];
+  for (int k = 0; k < V; ++k) x[k] = v[k];
+  *reinterpret_cast<vec*>(to) = x;
+}
+template <int V>
+__device__ __forceinline__ void add_row(float (&v)[V], const float* from) {
+  typedef float vec __attribute__((ext_vector_type(V)));
+  const vec x = *reinterpret_cast<const vec*>(from);
+#pragma unroll
+  for (int k = 0; k < V; ++k) v[k] += x[k];
 }
 // Four tokens of a lane's channel
 __device__ __forceinline__ f32x4 get_tokens(const float* tile, int t, int lane) {

@@ -78,10 +78,12 @@ __global__ __launch_bounds__(64 * (W + SSM_HELPERS), W == 8 ? 3 : 2) void ssm_bw
   const T* zb = has_z ? (const T*)p.z + at.b * p.z_b + last * z_t + at.c0 : nullptr;
   const T* dyb = (const T*)gr.dy + ((long long)at.b * p.L + last) * E + at.c0;
   const float* mb = p.mixed + ((long long)at.b * p.L + last) * E + at.c0;
-  RawRow<T, V, VEC> xr, dr, zr, yr;   // the next tile's rows
-  RawRow<float, V, VEC> mr;
-  struct Kept {                       // of a tile, from its beginning to its end
-    float x[V], dm[V], slope[V], dz[V];
+  struct Rows {   // of a tile
+    RawRow<T, V, VEC> x, dt, z, dy;
+    RawRow<float, V, VEC> mixed;
+  };
+  struct Kept {   // of a tile, from its beginning to its end
+    float x[V], delta[V], dm[V], slope[V], dz[V];
   };
   auto load_params = [&] {
 #pragma unroll
@@ -91,14 +93,14 @@ __global__ __launch_bounds__(64 * (W + SSM_HELPERS), W == 8 ? 3 : 2) void ssm_bw
       dD[i] = dbias[i] = 0.f;
     }
   };
-  auto load_rows = [&](int rows) {
-    const rsrc_t rx = open_rsrc(xb), rd = open_rsrc(db), rz = open_rsrc(zb), ry = open_rsrc(dyb);
-    if (!STATE) xr = load_raw<T, V, VEC>(rx, row * x_t + tc, row < rows, left);
-    dr = load_raw<T, V, VEC>(rd, row * dt_t + tc, row < rows, left);
-    zr = load_raw<T, V, VEC>(rz, row * z_t + tc, has_z && row < rows, left);
-    yr = load_raw<T, V, VEC>(ry, row * E + tc, row < rows, left);
+  auto load_rows = [&](int rows, Rows& r) {
+    const bool in = row < rows;
+    if (!STATE) r.x = load_raw<T, V, VEC>(open_rsrc(xb), row * x_t + tc, in, left);
+    r.dt = load_raw<T, V, VEC>(open_rsrc(db), row * dt_t + tc, in, left);
+    r.z = load_raw<T, V, VEC>(open_rsrc(zb), row * z_t + tc, has_z && in, left);
+    r.dy = load_raw<T, V, VEC>(open_rsrc(dyb), row * E + tc, in, left);
     if (!STATE) {
-      mr = load_raw<float, V, VEC>(open_rsrc(mb), row * E + tc, has_z && row < rows, left);
+      r.mixed = load_raw<float, V, VEC>(open_rsrc(mb), row * E + tc, has_z && in, left);
       mb -= SSM_TT * (long long)E;
     }
     xb -= SSM_TT * (long long)x_t;
@@ -106,34 +108,34 @@ __global__ __launch_bounds__(64 * (W + SSM_HELPERS), W == 8 ? 3 : 2) void ssm_bw
     if (has_z) zb -= SSM_TT * (long long)z_t;
     dyb -= SSM_TT * (long long)E;
   };
-  auto prep = [&](int rows, int buf, Kept& k) {
+  auto prep = [&](int rows, int buf, const Rows& r, Kept& k) {
     const int e = row * SSM_CH + tc;
-    float d[V], u[V];
+    float u[V];
 #pragma unroll
     for (int i = 0; i < V; ++i) {
-      const float pre = dr.at(i) + bias[i];
-      d[i] = pre, k.slope[i] = 1.f;
-      if (soft) d[i] = STATE ? softplus(pre) : softplus_slope(pre, k.slope[i]);
-      k.dm[i] = yr.at(i);
-      if (!STATE) k.x[i] = xr.at(i);
+      const float pre = r.dt.at(i) + bias[i];
+      k.delta[i] = pre, k.slope[i] = 1.f;
+      if (soft) k.delta[i] = STATE ? softplus(pre) : softplus_slope(pre, k.slope[i]);
+      k.dm[i] = r.dy.at(i);
+      if (!STATE) k.x[i] = r.x.at(i);
     }
     if (has_z) {
 #pragma unroll
       for (int i = 0; i < V; ++i) {
-        const float z = zr.at(i), s = sigmoid(z), dy = k.dm[i], zs = z * s;
+        const float z = r.z.at(i), s = sigmoid(z), dy = k.dm[i], zs = z * s;
         k.dm[i] = dy * zs;
-        if (!STATE) k.dz[i] = dy * mr.at(i) * fmaf(zs, 1.f - s, s);
+        if (!STATE) k.dz[i] = dy * r.mixed.at(i) * fmaf(zs, 1.f - s, s);
       }
     }
     if (rows < SSM_TT && row >= rows) {
 #pragma unroll
-      for (int i = 0; i < V; ++i) d[i] = 0.f;
+      for (int i = 0; i < V; ++i) k.delta[i] = 0.f;
     }
-    put_row(sd(buf) + e, d);
+    put_row(sd(buf) + e, k.delta);
     put_row(sg(buf) + e, k.dm);
     if (!STATE) {
 #pragma unroll
-      for (int i = 0; i < V; ++i) u[i] = d[i] * k.x[i];
+      for (int i = 0; i < V; ++i) u[i] = k.delta[i] * k.x[i];
       put_row(su(buf) + e, u);
     }
   };
@@ -169,12 +171,10 @@ __global__ __launch_bounds__(64 * (W + SSM_HELPERS), W == 8 ? 3 : 2) void ssm_bw
       return;
     }
     RawRow<T, V, VEC> ox, od, oz;
-    float d[V] = {0.f, 0.f, 0.f, 0.f};
-    add_row(d, sd(buf) + e);
 #pragma unroll
     for (int i = 0; i < V; ++i) {
       const float ddt = fmaf(k.x[i], sum[0][i], sum[1][i] * LN2) * k.slope[i];
-      ox.set(i, fmaf(d[i], sum[0][i], D[i] * k.dm[i]));
+      ox.set(i, fmaf(k.delta[i], sum[0][i], D[i] * k.dm[i]));
       od.set(i, ddt);
       if (has_z) oz.set(i, k.dz[i]);
       dD[i] = fmaf(k.dm[i], k.x[i], dD[i]);   // x and dy are zero where there is no row
@@ -319,23 +319,30 @@ __global__ __launch_bounds__(64 * (W + SSM_HELPERS), W == 8 ? 3 : 2) void ssm_bw
 
   const int t0 = at.tile0, t1 = at.tile1;   // t0 < t1
   if (wave >= W) {
-    Kept now, before;   // of this tile and the one after it in the sequence
+    // as in the forward, from the last tile on
+    Rows even, odd;
+    Kept now, last, before;
     load_params();
-    load_rows(rows_of(t1 - 1));
-    prep(rows_of(t1 - 1), 0, now);
-    if (t1 - 1 > t0) load_rows(SSM_TT);
+    load_rows(rows_of(t1 - 1), even);
+    if (t1 - 2 >= t0) load_rows(SSM_TT, odd);
+    prep(rows_of(t1 - 1), 0, even, now);
+    if (t1 - 3 >= t0) load_rows(SSM_TT, even);
     __syncthreads();
-    for (int tile = t1 - 1; tile >= t0; --tile) {
-      const int buf = (t1 - 1 - tile) & 1;
-      if (!STATE && tile < t1 - 1) finish(tile + 1, buf ^ 1, before);
+    auto step = [&](int tile, int buf, Rows& next) {
       before = now;
       if (tile > t0) {
-        prep(SSM_TT, buf ^ 1, now);
-        if (tile - 1 > t0) load_rows(SSM_TT);
+        prep(SSM_TT, buf ^ 1, next, now);
+        if (tile - 3 >= t0) load_rows(SSM_TT, next);
       }
+      if (!STATE && tile < t1 - 1) finish(tile + 1, buf ^ 1, last);
+      last = before;
       __syncthreads();
+    };
+    for (int tile = t1 - 1; tile >= t0; tile -= 2) {
+      step(tile, 0, odd);
+      if (tile > t0) step(tile - 1, 1, even);
     }
-    if (!STATE) finish(t0, (t1 - 1 - t0) & 1, before);
+    if (!STATE) finish(t0, (t1 - 1 - t0) & 1, last);
   } else {
     load_bc(rows_of(t1 - 1));
     next_bc();
