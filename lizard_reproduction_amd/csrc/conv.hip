@@ -34,15 +34,28 @@ struct ConvPlace {
   }
 };
 
-template <int K, int V>
+template <int K, int V, bool VEC>
 __device__ __forceinline__ void load_taps(const Conv& p, int col, int left, float (&w)[K][V],
                                           float (&bias)[V]) {
+  if constexpr (VEC) {   // the channels' taps lie next to each other
+    Cols<float, true, V * K> t;
+    t.load(p.w + (size_t)col * K, V * K);
+    Cols<float, true, V> b;
+    if (p.bias) b.load(p.bias + col, V);
 #pragma unroll
-  for (int i = 0; i < V; ++i) {
-    const int c = col + (i < left ? i : 0);
+    for (int i = 0; i < V; ++i) {
 #pragma unroll
-    for (int j = 0; j < K; ++j) w[j][i] = p.w[(size_t)c * K + j];
-    bias[i] = p.bias ? p.bias[c] : 0.f;
+      for (int j = 0; j < K; ++j) w[j][i] = t.r.at(i * K + j);
+      bias[i] = p.bias ? b.r.at(i) : 0.f;
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+      const int c = col + (i < left ? i : 0);
+#pragma unroll
+      for (int j = 0; j < K; ++j) w[j][i] = p.w[(size_t)c * K + j];
+      bias[i] = p.bias ? p.bias[c] : 0.f;
+    }
   }
 }
 
@@ -71,16 +84,23 @@ __global__ __launch_bounds__(CONV_THREADS) void conv_fwd_kernel(Conv p) {
   const T* xb = (const T*)p.x + at.b * p.x_b + at.col;
   T* yb = (T*)p.y + (long long)at.b * p.L * p.C + at.col;
   float w[K][V], bias[V], win[K][V];   // win[j]: row t - K + 1 + j
-  load_taps<K, V>(p, at.col, at.left, w, bias);
+  load_taps<K, V, VEC>(p, at.col, at.left, w, bias);
 #pragma unroll
   for (int j = 1; j < K; ++j)
     row_before<T, VEC, K, V>(p, xb, at.b, at.t0 + j - K, at.col, at.left, win[j]);
   const int t1 = min(at.t0 + p.run, p.L);
-  for (int t = at.t0; t < t1; t += CONV_AHEAD) {
-    Cols<T, VEC, V> next[CONV_AHEAD];
+  Cols<T, VEC, V> next[CONV_AHEAD];   // a batch of rows on its way while one is worked on
+  auto load = [&](int t) {
 #pragma unroll
     for (int i = 0; i < CONV_AHEAD; ++i)
       next[i].load(xb + (long long)min(t + i, p.L - 1) * p.x_t, at.left);
+  };
+  load(at.t0);
+  for (int t = at.t0; t < t1; t += CONV_AHEAD) {
+    Cols<T, VEC, V> x[CONV_AHEAD];
+#pragma unroll
+    for (int i = 0; i < CONV_AHEAD; ++i) x[i] = next[i];
+    if (t + CONV_AHEAD < t1) load(t + CONV_AHEAD);
 #pragma unroll
     for (int i = 0; i < CONV_AHEAD; ++i) {
       Cols<T, VEC, V> out;
@@ -88,7 +108,7 @@ __global__ __launch_bounds__(CONV_THREADS) void conv_fwd_kernel(Conv p) {
       for (int c = 0; c < V; ++c) {
 #pragma unroll
         for (int j = 0; j + 1 < K; ++j) win[j][c] = win[j + 1][c];
-        win[K - 1][c] = next[i].r.at(c);
+        win[K - 1][c] = x[i].r.at(c);
         float y = bias[c];
 #pragma unroll
         for (int j = 0; j < K; ++j) y = fmaf(w[j][c], win[j][c], y);
@@ -142,7 +162,7 @@ __global__ __launch_bounds__(CONV_THREADS) void conv_bwd_kernel(Conv p, const vo
   T* dxb = (T*)dx_ + (long long)at.b * p.L * p.C + at.col;
   float w[K][V], bias[V], win[K][V], g[K][V];   // g[j]: the gradient at token t - K + 1 + j
   float dw[K][V], dbias[V];
-  load_taps<K, V>(p, at.col, at.left, w, bias);
+  load_taps<K, V, VEC>(p, at.col, at.left, w, bias);
 #pragma unroll
   for (int c = 0; c < V; ++c) {
     dbias[c] = 0.f;
@@ -190,21 +210,27 @@ __global__ __launch_bounds__(CONV_THREADS) void conv_bwd_kernel(Conv p, const vo
     x.load(xb + r * p.x_t, at.left);
     dy.load(dyb + r * p.C, at.left);
   };
-  // A run is whole batches of rows, but the last one, whose rows past it are past the sequence
+  // A run is whole batches of rows, but the last one, whose rows past it are past the
+  // sequence; a batch is on its way while one is worked on
+  Cols<T, VEC, V> nx[CONV_AHEAD], ny[CONV_AHEAD];
+  auto load_batch = [&](int t) {
+#pragma unroll
+    for (int i = 0; i < CONV_AHEAD; ++i) load(t + i, nx[i], ny[i]);
+  };
+  static_assert(CONV_AHEAD >= CONV_MAX_TAPS - 1, "a batch holds the rows after a run");
   int t = at.t0;
+  load_batch(t);
   for (; t < t1; t += CONV_AHEAD) {
     Cols<T, VEC, V> x[CONV_AHEAD], dy[CONV_AHEAD];
 #pragma unroll
-    for (int i = 0; i < CONV_AHEAD; ++i) load(t + i, x[i], dy[i]);
+    for (int i = 0; i < CONV_AHEAD; ++i) x[i] = nx[i], dy[i] = ny[i];
+    load_batch(t + CONV_AHEAD);
 #pragma unroll
     for (int i = 0; i < CONV_AHEAD; ++i) row(t + i, x[i], dy[i], std::true_type());
   }
-  if (K > 1 && at.in) {   // the tokens after the run that its last rows reach
-    Cols<T, VEC, V> x[K], dy[K];
+  if (at.in) {   // the tokens after the run that its last rows reach
 #pragma unroll
-    for (int i = 0; i < K - 1; ++i) load(t + i, x[i], dy[i]);
-#pragma unroll
-    for (int i = 0; i < K - 1; ++i) row(t + i, x[i], dy[i], std::false_type());
+    for (int i = 0; i < K - 1; ++i) row(t + i, nx[i], ny[i], std::false_type());
   }
   // the workgroup's runs, one sum at a time: [K + 1][C] floats a row of workgroups
   const int runs = CONV_THREADS / p.cols;
@@ -234,6 +260,8 @@ void conv_split(Conv& p, bool backward) {
   const int V = backward ? CONV_BWD_V : CONV_FWD_V, vecs = (p.C + V - 1) / V;
   int cols = 1;
   while (cols < 64 && cols < vecs) cols *= 2;
+  // fewer where the last block of columns would be mostly empty
+  while (cols > 16 && (vecs + cols - 1) / cols * cols * 8 > vecs * 9) cols /= 2;
   p.cols = cols;
   p.col_blocks = (vecs + cols - 1) / cols;
   const long long rows = (long long)p.batch * p.L;

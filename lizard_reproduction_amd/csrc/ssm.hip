@@ -311,13 +311,10 @@ __global__ __launch_bounds__(256) void ssm_step_kernel(Ssm p, float* state) {
   }
 }
 
-#ifndef HELPERS
-#define HELPERS 8
-#endif
 template <typename T, int W, int NP, bool VEC>
 hipError_t fwd_launch(const Ssm& p, hipStream_t st) {
   const int nblk = p.G * p.gblocks;
-  constexpr int H = HELPERS;
+  constexpr int H = SSM_FWD_HELPERS;
   const dim3 block(64 * (W + H));
   if (p.S > 1) {
     hipLaunchKernelGGL((ssm_fwd_kernel<T, W, NP, H, VEC, true>), dim3(nblk * (p.S - 1) * p.batch),
@@ -341,15 +338,15 @@ hipError_t fwd_waves(const Ssm& p, hipStream_t st) {
 }
 
 // Segments of a sequence.  One where the 64-channel blocks fill the chip, as a pass over
-// the segments' own states costs half the walk again (B = 4, E = 4096, N = 16: 256 blocks;
-// two segments took the training pass from 730 to 816 us).  Else as many as bring the
-// forward to three workgroups a CU (B = 1, L = 2048, E = 4096: 86, 79, 80 and 84 us at one
-// to four; L = 16384, E = 2048: 346, 273, 260, 265), the backward, whose LDS leaves room for
-// one, to one; of four tiles at least.
+// the segments' own states costs half the walk again (training B = 4, E = 4096, N = 16, 256
+// blocks: two segments took 86 us more of 730).  Else as many as bring the forward to two
+// workgroups a CU (B = 1, L = 2048, E = 4096: 80, 76, 81 and 83 us at one to four; L =
+// 16384, E = 2048: 275, 244, 246, 249), the backward, whose LDS leaves room for one, to one;
+// of four tiles at least.
 int ssm_segments(int batch, int G, int Eg, int L, bool backward) {
   const int tiles = (L + SSM_TT - 1) / SSM_TT, cus = device_geom().cus;
   const long long groups = (long long)batch * G * ((Eg + SSM_CH - 1) / SSM_CH);
-  long long s = groups >= cus ? 1 : backward ? cus / groups : (3 * cus + groups - 1) / groups;
+  long long s = groups >= cus ? 1 : backward ? cus / groups : (2 * cus + groups - 1) / groups;
   if (s > tiles / 4) s = tiles / 4;
   if (s > 64) s = 64;
   if (s < 1) s = 1;
