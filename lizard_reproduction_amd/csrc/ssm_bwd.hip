@@ -11,7 +11,7 @@
 // as in the forward and walks the tiles from the last; in each it walks forward once, every
 // decay and state of its 16 tokens staying in registers, then back.  What is
 // summed over n meets in LDS, the waves' shares side by side; what is summed over channels
-// is added across the wave, two tokens' eight sums at a time, and its 64-channel shares, as the sequences' shares
+// is added across the wave, four tokens' sixteen sums at a time, and its 64-channel shares, as the sequences' shares
 // of dA, dD and dbias, go to memory for a second launch that adds them in
 // order: no atomics, the same bits every time.  More than 16 states are taken 16 a launch
 // (in one, a wave's registers did not hold them: N = 24 took 2.8 times as long as 16).
@@ -19,19 +19,29 @@
 
 namespace lz {
 
-// The sums of v0 .. v7 over the wave, each step halving the registers that carry them:
-// lane l gets sum l / 8.
-__device__ __forceinline__ float wave_sums8(const float (&v)[8]) {
-  float q[4], r[2];
-#pragma unroll
-  for (int k = 0; k < 4; ++k) q[k] = swap_add<false>(v[k], v[k + 4]);
-#pragma unroll
-  for (int k = 0; k < 2; ++k) r[k] = swap_add<true>(q[k], q[k + 2]);
-  // lanes 0 - 7 of a row go on with r[0], 8 - 15 with r[1]
-  const bool hi = threadIdx.x & 8;
-  float s = hi ? r[1] : r[0];
-  s += dpp<DPP_ROR8>(hi ? r[0] : r[1]);
-  s += dpp<DPP_HALF_MIRROR>(s);
+// The sums over the wave of v[0] .. v[15], each step halving the registers that carry them:
+// two values share a row of 16 lanes by its halves, four by its quads (a lane operand's sum
+// written to some banks of four lanes only, which takes no select: written out, with two
+// instructions at least from a register's write to its use as such an operand), then 8 and
+// 16 the wave by its rows.  Lane l gets v[4 (l / 16) + 2 (l / 4 % 2) + l / 8 % 2].  (36 issue
+// slots; by swaps and selects from the start, eight values at a time, 50.)
+__device__ __forceinline__ float wave_sums16(float (&v)[16]) {
+#define LZ_R8(d, s, m) "v_add_f32_dpp %" #d ", %" #s ", %" #s " row_ror:8 row_mask:0xf bank_mask:" #m "\n"
+#define LZ_HM(d, s, m) \
+  "v_add_f32_dpp %" #d ", %" #s ", %" #s " row_half_mirror row_mask:0xf bank_mask:" #m "\n"
+  asm("s_nop 1\n"
+      LZ_R8(0, 0, 0xf) LZ_R8(1, 1, 0xf) LZ_R8(2, 2, 0xf) LZ_R8(3, 3, 0xf)
+      LZ_R8(4, 4, 0xf) LZ_R8(5, 5, 0xf) LZ_R8(6, 6, 0xf) LZ_R8(7, 7, 0xf)
+      LZ_R8(0, 8, 0xc) LZ_R8(1, 9, 0xc) LZ_R8(2, 10, 0xc) LZ_R8(3, 11, 0xc)
+      LZ_R8(4, 12, 0xc) LZ_R8(5, 13, 0xc) LZ_R8(6, 14, 0xc) LZ_R8(7, 15, 0xc)
+      LZ_HM(0, 0, 0xf) LZ_HM(2, 2, 0xf) LZ_HM(4, 4, 0xf) LZ_HM(6, 6, 0xf)
+      LZ_HM(0, 1, 0xa) LZ_HM(2, 3, 0xa) LZ_HM(4, 5, 0xa) LZ_HM(6, 7, 0xa)
+      : "+&v"(v[0]), "+&v"(v[2]), "+&v"(v[4]), "+&v"(v[6]), "+&v"(v[8]), "+&v"(v[10]),
+        "+&v"(v[12]), "+&v"(v[14])
+      : "v"(v[1]), "v"(v[3]), "v"(v[5]), "v"(v[7]), "v"(v[9]), "v"(v[11]), "v"(v[13]), "v"(v[15]));
+#undef LZ_R8
+#undef LZ_HM
+  float s = swap_add<true>(swap_add<false>(v[0], v[8]), swap_add<false>(v[4], v[12]));
   s += dpp<DPP_XOR1>(s);
   s += dpp<DPP_XOR2>(s);
   return s;
@@ -254,7 +264,7 @@ __global__ __launch_bounds__(64 * (W + SSM_HELPERS), W == 8 ? 3 : 2) void ssm_bw
   auto scan = [&](int tile, int buf, bool more) {
     const int rows = rows_of(tile);
     const float Bf[2] = {Bv.at(0), Bv.at(1)}, Cf[2] = {Cv.at(0), Cv.at(1)}, hb[2] = {h0[0], h0[1]};
-    float a[16][2], h[16][2], bcsum = 0.f, v8[8];
+    float a[16][2], h[16][2], bcsum = 0.f;
     if (more) load_bc(SSM_TT);
     // forward over the tile
     static_for<16>([&](auto kt) {
@@ -272,34 +282,31 @@ __global__ __launch_bounds__(64 * (W + SSM_HELPERS), W == 8 ? 3 : 2) void ssm_bw
       constexpr int i = 3 - decltype(ki)::value, K = 8 * (i & 1);
       const f32x4 d4 = get_tokens(sd(buf), 4 * i, lane), u4 = get_tokens(su(buf), 4 * i, lane);
       const f32x4 g4 = get_tokens(sg(buf), 4 * i, lane);
-      float gs[4][2];
+      float gs[4][2], bc16[16];
       f32x4 dv = {0.f, 0.f, 0.f, 0.f}, du = {0.f, 0.f, 0.f, 0.f};
       static_for<4>([&](auto kt) {
-        constexpr int t = 3 - decltype(kt)::value, tt = 4 * i + t, to = tt & 1 ? 0 : 4;
+        constexpr int t = 3 - decltype(kt)::value, tt = 4 * i + t;
         ssm_fma2<K + 2 * t>(gs[t], Cf[i >> 1], g4[t], carry);
 #pragma unroll
         for (int n = 0; n < 2; ++n) {
           const float g = gs[t][n];
-          v8[to + n] = g * u4[t];
-          v8[to + 2 + n] = g4[t] * h[tt][n];
+          bc16[4 * t + n] = g * u4[t];
+          bc16[4 * t + 2 + n] = g4[t] * h[tt][n];
           carry[n] = a[tt][n] * g;
           const float v = carry[n] * (tt ? h[(tt + 15) % 16][n] : hb[n]);
           dv[t] = fmaf(v, A2[n], dv[t]);
           dA[n] = fmaf(v, d4[t], dA[n]);
         }
-        if (tt % 2 == 0) {   // tokens tt + 1 and tt
-          const float s = wave_sums8(v8);
-          if ((lane & 7) == tt / 2) bcsum = s;
-        }
       });
+      const float s = wave_sums16(bc16);
+      if ((lane & 3) == i) bcsum = s;
       ssm_dots<K>(du, Bf[i >> 1], gs);
       put_tokens(pd(buf, w), 4 * i, lane, dv);
       put_tokens(pu(buf, w), 4 * i, lane, du);
     });
-    // lane l: of token 2 (l % 8) + 1 (l < 32) or 2 (l % 8), B's or C's (l / 16 % 2), state
-    // l / 8 % 2
-    const int tk = 2 * (lane & 7) + (lane < 32);
-    const uint32_t off = (uint32_t)((2 * tk + (lane >> 4 & 1)) * NQ + n0 + (lane >> 3 & 1)) * 4u;
+    // lane l: of token 4 (l % 4) + l / 16, B's or C's (l / 4 % 2), state l / 8 % 2
+    const int tk = 4 * (lane & 3) + (lane >> 4);
+    const uint32_t off = (uint32_t)((2 * tk + (lane >> 2 & 1)) * NQ + n0 + (lane >> 3 & 1)) * 4u;
     __builtin_amdgcn_raw_buffer_store_b32(__builtin_bit_cast(uint32_t, bcsum), open_rsrc(bc),
                                           tk < rows ? off : OOB, 0, 0);
     bc -= SSM_TT * 2 * NQ;
