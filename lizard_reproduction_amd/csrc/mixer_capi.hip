@@ -32,12 +32,10 @@ int check_ssm_sizes(const char* what, long long batch, long long length, long lo
     return fail(1, "%s: %lld channels beyond %d unsupported", what, channels, LZ_MIXER_MAX_STRIDE);
   if (batch * length > ROWS_LIMIT)
     return fail(1, "%s: %lld tokens exceed the 2^31 - 2^20 limit", what, batch * length);
-  // workgroups of up to 768 threads, 64 segments a sequence; sums of 64 outputs
+  // workgroups of up to 1024 threads, segments only where there are fewer blocks than CUs
   const long long blocks = groups * ((channels / groups + 63) / 64);
-  if (batch * blocks > (1LL << 23) / 64 || batch > 65535)
+  if (batch * blocks > (1LL << 21) || batch > 65535)
     return fail(1, "%s: batch %lld x %lld blocks of channels exceed the grid", what, batch, blocks);
-  if (batch * length * state > (1LL << 29) || channels * state > (1LL << 29))
-    return fail(1, "%s: tokens x state (or channels x state) exceed 2^29", what);
   return 0;
 }
 

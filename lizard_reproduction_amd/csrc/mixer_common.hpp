@@ -222,14 +222,16 @@ __device__ __forceinline__ float lanes_sum(float v, int lanes) {
 }
 
 // Sums of partial results in the order of their index, by one launch.  A job sums, for
-// each of `rows` x `cols` outputs, `parts` values `part_stride` floats apart that begin
-// at src + row * row_stride + col; output (row, col) goes to
-// dst + row * out_row + col * out_col, as bf16 or float.
+// each of `sets` x `rows` x `cols` outputs, `parts` values `part_stride` floats apart that
+// begin at src + set * set_stride + row * row_stride + col; output (set, row, col) goes to
+// dst + set * out_set + row * out_row + col * out_col, as bf16 or float.
 struct SumJob {
   const float* src;
   void* dst;
   long long part_stride, row_stride, out_row, out_col;
   int rows, cols, parts, bf16;
+  int sets = 1;
+  long long set_stride = 0, out_set = 0;
 };
 constexpr int SUM_JOBS = 6;
 struct SumJobs {

@@ -8,6 +8,7 @@
 // of wider rows; anything else is copied.
 #include <c10/core/DeviceGuard.h>
 
+#include <limits>
 #include <optional>
 
 #include "torch_common.hpp"
@@ -28,18 +29,28 @@ at::ScalarType common(std::initializer_list<const Tensor*> tensors) {
 }
 
 // t itself where its last dimension is contiguous and the strides between are ones the
-// library takes, else a contiguous copy
-Tensor rows(const Tensor& t) {
+// library takes (up to `limit`), else a contiguous copy
+Tensor rows(const Tensor& t, int64_t limit = LZ_MIXER_MAX_STRIDE) {
   if (!t.defined()) return t;
   const int64_t last = t.dim() - 1;
   bool ok = t.size(last) <= 1 || t.stride(last) == 1;
-  for (int64_t d = 1; d < last; ++d) ok = ok && (t.size(d) <= 1 || t.stride(d) <= LZ_MIXER_MAX_STRIDE);
+  for (int64_t d = 1; d < last; ++d) ok = ok && (t.size(d) <= 1 || t.stride(d) <= limit);
   return ok ? t : t.contiguous();
 }
 
 // Elements from one entry of a dimension to the next; 0 where there is one entry
 long long step_of(const Tensor& t, int64_t d) {
   return t.defined() && t.size(d) > 1 ? t.stride(d) : 0;
+}
+
+// A backward may run on a stream that is being captured though its forward ran eagerly:
+// refused, as kernels.py refuses the calls
+void refuse_capture(const Tensor& t) {
+  hipStreamCaptureStatus status = hipStreamCaptureStatusNone;
+  if (hipStreamIsCapturing(static_cast<hipStream_t>(stream_of(t)), &status) != hipSuccess ||
+      status != hipStreamCaptureStatusNone)
+    throw std::runtime_error("lizard_reproduction_amd kernels: calls under HIP graph capture are "
+                             "not supported (run the kernels eagerly)");
 }
 
 // Contiguous, of t's sizes and type; not given where t is not
@@ -131,10 +142,9 @@ struct SsmNode : torch::autograd::Function<SsmNode> {
         {static_cast<int64_t>(lz_ssm_states_bytes(a.batch, a.length, a.channels, a.state, a.z != nullptr) / 4)},
         c.A.options());
     const Tensor y = c.forward({}, {}, {}, states);
-    ctx->save_for_backward({c.x, c.dt, c.A, c.B, c.C, c.D, c.z, c.bias});
+    ctx->save_for_backward({c.x, c.dt, c.A, c.B, c.C, c.D, c.z, c.bias, states});
     ctx->saved_data["types"] = types({&x, &dt, &A, &B, &C, &D, &z, &bias});
     ctx->saved_data["softplus"] = softplus;
-    ctx->saved_data["states"] = states;
     return y.to(x.scalar_type());
   }
 
@@ -142,8 +152,9 @@ struct SsmNode : torch::autograd::Function<SsmNode> {
     const variable_list s = ctx->get_saved_variables();
     const SsmCall c{s[0], s[1], s[2], s[3], s[4], s[5], s[6], s[7],
                     ctx->saved_data["softplus"].toBool()};
-    const Tensor states = ctx->saved_data["states"].toTensor();
+    const Tensor& states = s[8];
     const c10::DeviceGuard guard(c.x.device());
+    refuse_capture(c.x);
     const lz_ssm_args a = c.args();
     const Tensor dy = upstream(grads[0], c.x);
     const Tensor dx = like(c.x), ddt = like(c.dt), dA = like(c.A),
@@ -294,6 +305,7 @@ struct ConvNode : torch::autograd::Function<ConvNode> {
     const variable_list s = ctx->get_saved_variables();
     const ConvCall c{s[0], s[1], s[2], ctx->saved_data["silu"].toBool()};
     const c10::DeviceGuard guard(c.x.device());
+    refuse_capture(c.x);
     const Tensor dy = upstream(grads[0], c.x);
     const Tensor dx = like(c.x), dw = like(c.w), dbias = like(c.bias);
     const int b = i32(c.x.size(0)), n = i32(c.x.size(1)), ch = i32(c.x.size(2)), k = i32(c.w.size(1));
@@ -400,7 +412,8 @@ struct NormCall {
 NormCall norm_call(const Tensor& x, const Tensor& w, const Tensor& bias, const Tensor& gate,
                    bool silu, double eps) {
   const auto t = common({&x, &gate});
-  return {rows(cast(x, t)), params(w), params(bias), rows(cast(gate, t)), silu, eps};
+  const int64_t any = std::numeric_limits<int64_t>::max();
+  return {rows(cast(x, t), any), params(w), params(bias), rows(cast(gate, t), any), silu, eps};
 }
 
 struct NormNode : torch::autograd::Function<NormNode> {
@@ -421,6 +434,7 @@ struct NormNode : torch::autograd::Function<NormNode> {
     const NormCall c{s[0], s[1], s[2], s[3], ctx->saved_data["silu"].toBool(),
                      ctx->saved_data["eps"].toDouble()};
     const c10::DeviceGuard guard(c.x.device());
+    refuse_capture(c.x);
     const lz_group_norm_args a = c.args();
     const Tensor dy = upstream(grads[0], c.x);
     const Tensor dx = like(c.x), dgate = like(c.gate), dw = like(c.w),

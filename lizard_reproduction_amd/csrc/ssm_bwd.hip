@@ -210,23 +210,23 @@ __global__ __launch_bounds__(64 * (W + SSM_HELPERS), W == 8 ? 3 : 2) void ssm_bw
   float h0[2];
   auto start = [&] {
 #pragma unroll
-      for (int k = 0; k < 2; ++k) {
-        const int n = n0 + k;
-        A2[k] = mine && n < N ? p.A[(size_t)c * N + n] * LOG2E : 0.f;
-        carry[k] = dA[k] = 0.f;
-      }
+    for (int k = 0; k < 2; ++k) {
+      const int n = n0 + k;
+      A2[k] = mine && n < N ? p.A[(size_t)c * N + n] * LOG2E : 0.f;
+      carry[k] = dA[k] = 0.f;
+    }
     if constexpr (!STATE) {
       // what the later segments carry back
       for (int j = p.S - 1; j > at.s; --j) {
         const size_t rec = (size_t)at.b * (p.S - 1) + j - 1;
         const float d = mine ? gr.dsum[rec * E + c] : 0.f;
 #pragma unroll
-          for (int k = 0; k < 4; ++k) {
-            const int n = n0 + k;
-            if (mine && n < N)
-              carry[k] = fmaf(__builtin_amdgcn_exp2f(A2[k] * d), carry[k],
-                                 gr.rec[(rec * N + n) * E + c]);
-          }
+        for (int k = 0; k < 2; ++k) {
+          const int n = n0 + k;
+          if (mine && n < N)
+            carry[k] = fmaf(__builtin_amdgcn_exp2f(A2[k] * d), carry[k],
+                            gr.rec[(rec * N + n) * E + c]);
+        }
       }
     }
   };
@@ -433,24 +433,18 @@ hipError_t launch_ssm_bwd(const Ssm& p, const SsmGrad& gr, void* dB, void* dC, f
   if (e != hipSuccess) return e;
   const int NQ = gr.NQ, parts = p.batch * p.S;
   const long long rows = (long long)p.batch * p.L;
-  // dB and dC: the blocks of a group, for each group
-  for (int g0 = 0; g0 < p.G; g0 += SUM_JOBS / 2) {
-    SumJobs jobs = {};
-    for (int g = g0; g < p.G && g < g0 + SUM_JOBS / 2; ++g)
-      for (int k = 0; k < 2; ++k) {
-        SumJob& j = jobs.job[jobs.n++];
-        j.src = gr.part_bc + (long long)g * p.gblocks * rows * 2 * NQ + k * NQ;
-        void* const dst = k ? dC : dB;
-        j.dst = is_bf16 ? (void*)((bf16*)dst + g * p.N) : (void*)((float*)dst + g * p.N);
-        j.part_stride = rows * 2 * NQ;
-        j.row_stride = 2 * NQ;
-        j.out_row = (long long)p.G * p.N;
-        j.out_col = 1;
-        j.rows = (int)rows, j.cols = p.N, j.parts = p.gblocks, j.bf16 = is_bf16;
-      }
-    if (e = launch_sums(jobs, st); e != hipSuccess) return e;
-  }
   SumJobs jobs = {};
+  for (int k = 0; k < 2; ++k) {   // dB and dC: the blocks of a group, for each group
+    SumJob& j = jobs.job[jobs.n++];
+    j.src = gr.part_bc + k * NQ;
+    j.dst = k ? dC : dB;
+    j.part_stride = rows * 2 * NQ;
+    j.row_stride = 2 * NQ;
+    j.out_row = (long long)p.G * p.N;
+    j.out_col = 1;
+    j.rows = (int)rows, j.cols = p.N, j.parts = p.gblocks, j.bf16 = is_bf16;
+    j.sets = p.G, j.set_stride = p.gblocks * rows * 2 * NQ, j.out_set = p.N;
+  }
   jobs.job[jobs.n++] = SumJob{gr.part_a, dA, (long long)p.N * p.E, p.E, 1, p.N, p.N, p.E, parts, 0};
   for (int k = 0; k < 2; ++k)
     if (float* dst = k ? dbias : dD)

@@ -10,46 +10,60 @@ namespace lz {
 
 constexpr int SUM_WAVES = 8, SUM_BATCH = 8;
 
+constexpr int SUM_GRID = 1 << 22;   // workgroups; more outputs are taken in rounds
+
 struct SumGrid {
   SumJobs jobs;
-  int blk0[SUM_JOBS + 1];
+  long long blk0[SUM_JOBS + 1];
 };
 
 __global__ __launch_bounds__(64 * SUM_WAVES) void sums_kernel(SumGrid g) {
   __shared__ float red[SUM_WAVES][64];
-  int j = 0;
-#pragma unroll
-  for (int i = 1; i < SUM_JOBS; ++i)
-    if (i < g.jobs.n && (int)blockIdx.x >= g.blk0[i]) j = i;
-  const SumJob& q = g.jobs.job[j];
   const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
-  const long long at = (long long)((int)blockIdx.x - g.blk0[j]) * 64 + lane;
-  const bool in = at < (long long)q.rows * q.cols;
-  const long long row = in ? at / q.cols : 0;
-  const int col = in ? (int)(at - row * q.cols) : 0;
-  const float* src = q.src + row * q.row_stride + col;
-  const int run = (q.parts + SUM_WAVES - 1) / SUM_WAVES;
-  const int end = min(q.parts, (wave + 1) * run);
-  float sum = 0.f;
-  if (in)
-    for (int p = wave * run; p < end; p += SUM_BATCH) {
-      float v[SUM_BATCH];
+  for (long long blk = blockIdx.x; blk < g.blk0[g.jobs.n]; blk += SUM_GRID) {
+    int j = 0;
 #pragma unroll
-      for (int k = 0; k < SUM_BATCH; ++k)
-        v[k] = src[(long long)min(p + k, end - 1) * q.part_stride];
-#pragma unroll
-      for (int k = 0; k < SUM_BATCH; ++k) sum += p + k < end ? v[k] : 0.f;
+    for (int i = 1; i < SUM_JOBS; ++i)
+      if (i < g.jobs.n && blk >= g.blk0[i]) j = i;
+    const SumJob& q = g.jobs.job[j];
+    const long long at = (blk - g.blk0[j]) * 64 + lane;
+    const bool in = at < (long long)q.sets * q.rows * q.cols;
+    long long row = in ? at / q.cols : 0;
+    const int col = in ? (int)(at - row * q.cols) : 0;
+    const float* src = q.src + col;
+    long long out = col * q.out_col;
+    if (q.sets > 1) {
+      const long long set = row / q.rows;
+      row -= set * q.rows;
+      src += set * q.set_stride;
+      out += set * q.out_set;
     }
-  red[wave][lane] = sum;
-  __syncthreads();
-  if (wave || !in) return;
+    src += row * q.row_stride;
+    out += row * q.out_row;
+    const int run = (q.parts + SUM_WAVES - 1) / SUM_WAVES;
+    const int end = min(q.parts, (wave + 1) * run);
+    float sum = 0.f;
+    if (in)
+      for (int p = wave * run; p < end; p += SUM_BATCH) {
+        float v[SUM_BATCH];
 #pragma unroll
-  for (int w = 1; w < SUM_WAVES; ++w) sum += red[w][lane];
-  const long long out = row * q.out_row + col * q.out_col;
-  if (q.bf16)
-    static_cast<bf16*>(q.dst)[out] = to_bf16(sum);
-  else
-    static_cast<float*>(q.dst)[out] = sum;
+        for (int k = 0; k < SUM_BATCH; ++k)
+          v[k] = src[(long long)min(p + k, end - 1) * q.part_stride];
+#pragma unroll
+        for (int k = 0; k < SUM_BATCH; ++k) sum += p + k < end ? v[k] : 0.f;
+      }
+    red[wave][lane] = sum;
+    __syncthreads();
+    if (wave == 0 && in) {
+#pragma unroll
+      for (int w = 1; w < SUM_WAVES; ++w) sum += red[w][lane];
+      if (q.bf16)
+        static_cast<bf16*>(q.dst)[out] = to_bf16(sum);
+      else
+        static_cast<float*>(q.dst)[out] = sum;
+    }
+    __syncthreads();
+  }
 }
 
 hipError_t launch_sums(const SumJobs& jobs, hipStream_t st) {
@@ -57,12 +71,14 @@ hipError_t launch_sums(const SumJobs& jobs, hipStream_t st) {
   g.jobs = jobs;
   long long blocks = 0;
   for (int i = 0; i < jobs.n; ++i) {
-    g.blk0[i] = (int)blocks;
-    blocks += ((long long)jobs.job[i].rows * jobs.job[i].cols + 63) / 64;
+    const SumJob& q = jobs.job[i];
+    g.blk0[i] = blocks;
+    blocks += ((long long)q.sets * q.rows * q.cols + 63) / 64;
   }
+  g.blk0[jobs.n] = blocks;
   if (!blocks) return hipSuccess;
-  if (blocks >= (1LL << 31)) return hipErrorInvalidValue;
-  hipLaunchKernelGGL(sums_kernel, dim3((unsigned)blocks), dim3(64 * SUM_WAVES), 0, st, g);
+  const unsigned grid = (unsigned)(blocks < SUM_GRID ? blocks : SUM_GRID);
+  hipLaunchKernelGGL(sums_kernel, dim3(grid), dim3(64 * SUM_WAVES), 0, st, g);
   return hipGetLastError();
 }
 

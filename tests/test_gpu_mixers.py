@@ -139,6 +139,130 @@ def test_ssm_segments(length, e, n, dtype):
     _check_ssm(c, dy, label=f"ssm segments L={length}")
 
 
+def test_ssm_many_groups():
+    """More groups than a launch of sums has jobs, of widths under a vector and over."""
+    for e, groups, n in ((40, 20, 16), (60, 5, 3), (70, 7, 18)):
+        _check_ssm(*_ssm_inputs(2, 21, e, n, groups, dtype=BF16, seed=groups),
+                   label=f"ssm E={e} G={groups}")
+
+
+@pytest.mark.parametrize("z", [True, False])
+@pytest.mark.parametrize("e, groups, n, dtype", [(33, 1, 34, BF16), (21, 3, 16, FP32), (6, 2, 5, BF16),
+                                                 (65, 1, 2, FP32)])
+def test_ssm_segments_of_odd_channels(e, groups, n, dtype, z):
+    """Split walks whose channels are no whole vectors, with states in several launches."""
+    c, dy = _ssm_inputs(2, 395, e, n, groups, dtype=dtype, z=z, seed=e)
+    c["dt_bias"] = c["dt_bias"] - 3
+    _check_ssm(c, dy, label=f"ssm odd segments E={e}")
+
+
+def test_ssm_more_sums_than_a_launch():
+    """So many tokens that dB's and dC's sums take several rounds of their launch: each
+    sequence's gradients are those of a call of its own, whose sums take one."""
+    b, length, n = 3, 2 ** 20, 64
+    assert 2 * b * length * n > 64 * 2 ** 22 >= 2 * length * n
+    g = torch.Generator("cuda").manual_seed(0)
+    c = {k: torch.randn(*shape, device="cuda", dtype=BF16, generator=g)
+         for k, shape in dict(x=(b, length, 1), dt=(b, length, 1), B=(b, length, n), C=(b, length, n)).items()}
+    A = -torch.rand(1, n, device="cuda", generator=g)
+    dy = torch.randn(b, length, 1, device="cuda", dtype=BF16, generator=g)
+
+    def grads(lo, hi):
+        leaves = {k: v[lo:hi].detach().requires_grad_() for k, v in c.items()}
+        return _backward(kernels.ssm(A=A, **leaves), leaves, dy[lo:hi])
+    whole = grads(0, b)
+    for i in range(b):
+        for k, grad in grads(i, i + 1).items():
+            assert torch.equal(grad, whole[k][i:i + 1]), (i, k)
+
+
+def _far(t, token):
+    """The same values, tokens `token` elements apart in memory that nothing else fills."""
+    b, length, *rest = t.shape
+    wide = torch.empty(b * length * token, device="cuda", dtype=t.dtype)
+    inner = torch.empty(rest).stride()
+    out = wide.as_strided(t.shape, (length * token, token, *inner))
+    out.copy_(t)
+    return out
+
+
+def test_rows_far_apart():
+    """Offsets past 32 bits, in elements and in bytes, at the largest token stride taken as
+    it is and at one past it (copied)."""
+    c, dy = _ssm_inputs(2, 70, 64, 16, 2, dtype=BF16)
+    gpu = {k: _cuda(v) for k, v in c.items()}
+    w = _randn(_gen(1), 64, 4).cuda()
+    nw = _randn(_gen(2), 64).cuda()
+    limit = 2 ** 24
+    assert 2 * 70 * limit > 2 ** 31
+
+    def run(x, z):
+        out = []
+        leaves = dict(x=x.detach().requires_grad_(), z=z.detach().requires_grad_())
+        for y in (kernels.ssm(**dict(gpu, **leaves)),
+                  kernels.short_conv(leaves["x"], w),
+                  kernels.group_norm(leaves["x"], 4, nw, gate=leaves["z"])):
+            out += [y, *torch.autograd.grad(y, list(leaves.values()), dy.cuda(), allow_unused=True)]
+        return out
+    want = run(gpu["x"], gpu["z"])
+    for token in (limit, limit + 1):
+        x = _far(gpu["x"], token)
+        for a, b in zip(run(x, gpu["z"]), want):
+            assert (a is None and b is None) or torch.equal(a, b), token
+        del x
+        z = _far(gpu["z"], token)
+        for a, b in zip(run(gpu["x"], z), want):
+            assert (a is None and b is None) or torch.equal(a, b), token
+        del z
+    B = _far(gpu["B"], limit)
+    assert torch.equal(kernels.ssm(**dict(gpu, B=B)), want[0])
+
+
+def test_steps_of_operands_in_any_form():
+    """Operands that a step's launch does not take as they are: strided, of other types, with
+    parameters in bf16, in one group or several."""
+    for groups, n in ((1, 16), (2, 5), (3, 64)):
+        c, _ = _ssm_inputs(3, 1, 66, n, groups, seed=n)
+        h0 = _randn(_gen(n), 3, 66, n)
+        want = ref.ssm(**c, state=h0)
+        at = {k: v[:, 0] if v.dim() > 2 else v for k, v in c.items()}
+        if groups == 1:
+            at["B"], at["C"] = at["B"][:, 0], at["C"][:, 0]
+        for form in ("whole", "slice", "half", "strided"):
+            for names in (list(at), ["x"], ["dt", "A"], ["B", "D"], ["C", "z", "dt_bias"]):
+                h = h0.cuda()
+                y = kernels.ssm_decode_step(**{k: _layout(v, form if k in names else "whole")
+                                               for k, v in at.items()}, state=h)
+                check(y, *(t[:, 0] for t in want["y"]), 264, f"step {form}")
+                check(h, *want["state"], 264, f"step state {form}")
+    c, _ = _ssm_inputs(2, 1, 64, 16, dtype=BF16)
+    c["dt"] = c["dt"].float() + 0.001
+    c["A"] = c["A"].to(BF16)
+    c["D"] = c["D"].double().float().to(BF16)
+    h0 = _randn(_gen(1), 2, 64, 16)
+    want = ref.ssm(**c, state=h0)
+    h = h0.cuda()
+    y = kernels.ssm_decode_step(**{k: v.cuda()[:, 0] if v.dim() > 2 else v.cuda() for k, v in c.items()},
+                                state=h)
+    assert y.dtype == BF16
+    check(y, *(t[:, 0] for t in want["y"]), 264, "step mixed")
+    check(h, *want["state"], 264, "step mixed state")
+
+
+def test_steps_write_their_state_alone():
+    """States as slots of a larger cache: the slots beside them stay as they were."""
+    cache = torch.randn(5, 64, 16, device="cuda")
+    rows = torch.randn(5, 3, 64, device="cuda")
+    kept, kept_rows = cache.clone(), rows.clone()
+    c, _ = _ssm_inputs(2, 1, 64, 16)
+    at = {k: v.cuda()[:, 0] if v.dim() > 2 else v.cuda() for k, v in c.items()}
+    kernels.ssm_decode_step(**at, state=cache[1:3])
+    kernels.short_conv_decode_step(at["x"], torch.ones(64, 4, device="cuda"), rows[1:3])
+    for now, before in ((cache, kept), (rows, kept_rows)):
+        assert torch.equal(now[:1], before[:1]) and torch.equal(now[3:], before[3:])
+        assert not torch.equal(now[1:3], before[1:3])
+
+
 def test_ssm_mixed_types():
     """An fp32 operand among bf16 ones: computed in fp32, returned in x's type."""
     c, dy = _ssm_inputs(2, 20, 48, 16, dtype=BF16)
@@ -300,6 +424,12 @@ def test_conv_channels(c, act, bias):
         _check_conv(3, 41, c, 4, act, bias, dtype, seed=c)
 
 
+def test_conv_widest_rows():
+    """As many channels as are taken, one past a vector less, forward and back."""
+    for c, taps in ((2 ** 24, 2), (2 ** 24 - 7, 1)):
+        _check_conv(1, 1, c, taps, True, False, BF16)
+
+
 @pytest.mark.parametrize("form", ["slice", "half", "swapped", "strided"])
 def test_conv_layouts(form):
     for dtype in (BF16, FP32):
@@ -414,6 +544,29 @@ def test_norm_of_attention_heads():
     got = kernels.group_norm(y.transpose(1, 2), None, activation=None)
     want = ref.norm(y.transpose(1, 2).flatten(-2), 5, act=False)["y"]
     check(got.flatten(-2), *want, 96, "norm heads")
+
+
+@pytest.mark.parametrize("which", ["weight", "bias"])
+def test_norm_weight_or_bias_alone(which):
+    g = _gen(3)
+    x, p, dy = _randn(g, 3, 7, 48), _randn(g, 48), _randn(g, 3, 7, 48)
+    leaves = {"x": x.cuda().requires_grad_(), which: p.cuda().requires_grad_()}
+    y = kernels.group_norm(groups=3, **leaves)
+    grads = _backward(y, leaves, dy.cuda())
+    want = ref.norm(x, 3, *((p, None) if which == "weight" else (None, p)), dy=dy)
+    check(y, *want["y"], 64, f"norm {which} alone y")
+    for k, grad in grads.items():
+        check(grad, *want["d" + k], 128 + 21, f"norm {which} alone d{k}")
+
+
+def test_norm_heads_far_apart():
+    """Heads further apart than tokens may be: a long attention output, heads first."""
+    x = torch.randn(2, 3, 5, 64, device="cuda", dtype=BF16)          # [B, H, L, D]
+    wide = torch.empty(2 * 3 * 2 ** 25, device="cuda", dtype=BF16)
+    far = wide.as_strided(x.shape, (3 * 2 ** 25, 2 ** 25, 64, 1))
+    far.copy_(x)
+    assert torch.equal(kernels.group_norm(far.transpose(1, 2), None),
+                       kernels.group_norm(x.transpose(1, 2), None))
 
 
 def test_norm_many_rows():
@@ -572,7 +725,7 @@ def test_some_inputs_without_gradients_and_autograd_features():
             y = call(**leaves)
         for a, b in zip(torch.autograd.grad(y, list(leaves.values()), dy), whole[1:]):
             assert torch.equal(a, b)
-        assert len(packed) == len(leaves)
+        assert len(packed) == len(leaves) + (call is kernels.ssm)     # and the scan's states
         with pytest.raises(RuntimeError, match="second time"):
             torch.autograd.grad(y, list(leaves.values()), dy)
         y = call(**leaves)

@@ -11,6 +11,12 @@ from tests import mixers_reference as ref
 from tests.test_capi import lib, no_gpu, refused  # noqa: F401  (lib: a fixture)
 
 
+@pytest.fixture(autouse=True)
+def gpu_as_it_is(monkeypatch):
+    """The presence of a GPU asked anew (kernels.py remembers one, and other tests say so)."""
+    monkeypatch.setattr(kernels, "_GPU_SEEN", False)
+
+
 def _randn(g, *shape):
     return torch.randn(shape, generator=g, dtype=torch.float64)
 
