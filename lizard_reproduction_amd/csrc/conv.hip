@@ -104,6 +104,7 @@ __global__ __launch_bounds__(CONV_THREADS) void conv_fwd_kernel(Conv p) {
 #pragma unroll
     for (int i = 0; i < CONV_AHEAD; ++i) {
       Cols<T, VEC, V> out;
+      float ys[V];
 #pragma unroll
       for (int c = 0; c < V; ++c) {
 #pragma unroll
@@ -113,8 +114,9 @@ __global__ __launch_bounds__(CONV_THREADS) void conv_fwd_kernel(Conv p) {
 #pragma unroll
         for (int j = 0; j < K; ++j) y = fmaf(w[j][c], win[j][c], y);
         if (p.act) y *= sigmoid(y);
-        out.r.set(c, t + i < len ? y : 0.f);
+        ys[c] = t + i < len ? y : 0.f;
       }
+      out.r.pack(ys);
       if (t + i < t1) out.store(yb + (long long)(t + i) * p.C, at.left);
     }
   }
@@ -125,8 +127,7 @@ __global__ __launch_bounds__(CONV_THREADS) void conv_fwd_kernel(Conv p) {
       float v[V];
       row_before<T, VEC, K, V>(p, xb, at.b, len - (K - 1) + j, at.col, at.left, v);
       Cols<T, VEC, V> out;
-#pragma unroll
-      for (int c = 0; c < V; ++c) out.r.set(c, v[c]);
+      out.r.pack(v);
       out.store((T*)p.state_out + ((long long)at.b * (K - 1) + j) * p.C + at.col, at.left);
     }
   }
@@ -177,6 +178,7 @@ __global__ __launch_bounds__(CONV_THREADS) void conv_bwd_kernel(Conv p, const vo
   const int t1 = at.in ? min(at.t0 + p.run, p.L) : at.t0;
   auto row = [&](int t, const Cols<T, VEC, V>& x, const Cols<T, VEC, V>& dy, auto own) {
     Cols<T, VEC, V> out;
+    float dxs[V];
     const bool there = t < p.L;
 #pragma unroll
     for (int c = 0; c < V; ++c) {
@@ -200,8 +202,9 @@ __global__ __launch_bounds__(CONV_THREADS) void conv_bwd_kernel(Conv p, const vo
         if (decltype(own)::value) dw[j][c] = fmaf(d, win[j][c], dw[j][c]);
         dx = fmaf(w[j][c], g[K - 1 - j][c], dx);   // g at token t - j: tap K - 1 - j
       }
-      out.r.set(c, dx);
+      dxs[c] = dx;
     }
+    out.r.pack(dxs);
     const int to = t - (K - 1);
     if (to >= at.t0 && to < t1) out.store(dxb + (long long)to * p.C, at.left);
   };

@@ -22,14 +22,17 @@ struct RawRow {
     else if constexpr (!VEC) return __builtin_bit_cast(float, w[i] << 16);
     else return __builtin_bit_cast(float, (i & 1) ? w[i >> 1] & 0xffff0000u : w[i >> 1] << 16);
   }
-  __device__ __forceinline__ void set(int i, float x) {
-    if constexpr (!IS_BF16<T>) {
-      w[i] = __builtin_bit_cast(uint32_t, x);
-    } else {
-      const uint32_t h = __builtin_bit_cast(uint16_t, to_bf16(x));
-      if constexpr (!VEC) w[i] = h;
-      else if (i & 1) w[i >> 1] |= h << 16;
-      else w[i >> 1] = h;
+  // rounded once, two to an instruction where they are packed
+  __device__ __forceinline__ void pack(const float (&x)[V]) {
+    typedef bf16 pair __attribute__((ext_vector_type(2)));
+#pragma unroll
+    for (int i = 0; i < WORDS; ++i) {
+      if constexpr (!IS_BF16<T>)
+        w[i] = __builtin_bit_cast(uint32_t, x[i]);
+      else if constexpr (!VEC || V == 1)
+        w[i] = __builtin_bit_cast(uint16_t, to_bf16(x[i]));
+      else
+        w[i] = __builtin_bit_cast(uint32_t, pair{to_bf16(x[2 * i]), to_bf16(x[2 * i + 1])});
     }
   }
 };
@@ -210,15 +213,32 @@ __device__ __forceinline__ float swap_add(float a, float b) {
   return __builtin_bit_cast(float, lo) + __builtin_bit_cast(float, hi);
 }
 
-// The sum over each `lanes` (a power of two, uniform) consecutive lanes, in all of them
-__device__ __forceinline__ float lanes_sum(float v, int lanes) {
-  if (lanes > 1) v += dpp<DPP_XOR1>(v);
-  if (lanes > 2) v += dpp<DPP_XOR2>(v);
-  if (lanes > 4) v += dpp<DPP_HALF_MIRROR>(v);
-  if (lanes > 8) v += dpp<DPP_MIRROR>(v);
-  if (lanes > 16) v = swap_add<true>(v, v);
-  if (lanes > 32) v = swap_add<false>(v, v);
-  return v;
+// The sums over each `lanes` (a power of two, uniform) consecutive lanes, in all of them.
+// (The empty asm has the comparisons made where they are: kept from before a loop, they come
+// out of vector registers.)
+template <int N>
+__device__ __forceinline__ void lanes_sum(float (&v)[N], int lanes) {
+  asm volatile("" : "+s"(lanes));
+  auto add = [&](auto other) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) v[i] = other(v[i]);
+  };
+  auto quads = [&] {
+    add([](float x) { return x + dpp<DPP_XOR1>(x); });
+    add([](float x) { return x + dpp<DPP_XOR2>(x); });
+  };
+  if (lanes >= 16) {
+    quads();
+    add([](float x) { return x + dpp<DPP_HALF_MIRROR>(x); });
+    add([](float x) { return x + dpp<DPP_MIRROR>(x); });
+    if (lanes >= 32) add([](float x) { return swap_add<true>(x, x); });
+    if (lanes >= 64) add([](float x) { return swap_add<false>(x, x); });
+  } else if (lanes >= 4) {
+    quads();
+    if (lanes >= 8) add([](float x) { return x + dpp<DPP_HALF_MIRROR>(x); });
+  } else if (lanes >= 2) {
+    add([](float x) { return x + dpp<DPP_XOR1>(x); });
+  }
 }
 
 // Sums of partial results in the order of their index, by one launch.  A job sums, for

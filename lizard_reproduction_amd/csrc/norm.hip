@@ -19,18 +19,23 @@
 
 namespace lz {
 
-// Sum over the tpg threads of a group (a power of two; past a wave through LDS)
-__device__ __forceinline__ float group_sum(float v, int tpg, float* red) {
-  v = lanes_sum(v, tpg);
+// Sums over the tpg threads of a group (a power of two; past a wave through LDS)
+template <int S>
+__device__ __forceinline__ void group_sums(float (&v)[S], int tpg, float (&red)[S][4]) {
+  lanes_sum(v, tpg);
   if (tpg > 64) {   // uniform
     const int wave = threadIdx.x >> 6, per = tpg >> 6;
     __syncthreads();
-    if ((threadIdx.x & 63) == 0) red[wave] = v;
+#pragma unroll
+    for (int k = 0; k < S; ++k)
+      if ((threadIdx.x & 63) == 0) red[k][wave] = v[k];
     __syncthreads();
-    v = 0.f;
-    for (int i = 0; i < per; ++i) v += red[wave / per * per + i];
+#pragma unroll
+    for (int k = 0; k < S; ++k) {
+      v[k] = 0.f;
+      for (int i = 0; i < per; ++i) v[k] += red[k][wave / per * per + i];
+    }
   }
-  return v;
 }
 
 // How a thread's vectors meet the group's channels: FULL, the threads' vectors are the
@@ -63,46 +68,38 @@ struct NormPlace {
   __device__ __forceinline__ bool has(int j, int i) const { return FIT == FULL || own[j] >> i & 1; }
 };
 
-// Rows of a tensor of groups, `step` apart, past the last one the last
-template <typename T>
-struct NormRows {
-  const T *p, *last;
-  long long step, wrap;   // elements from a row to the next, and more where that passes a sequence
+// A walk over rows `step` apart in x and the gate, past the last one the last
+template <typename T, bool GATE>
+struct NormWalk {
+  static constexpr int M = GATE ? 2 : 1;
+  const T *p[M], *last[M];
+  long long step[M], wrap[M];   // elements to the next row, and more where that passes a sequence
   int left, t, step_t, L;
-  __device__ __forceinline__ NormRows(const void* base, long long sb, long long st, long long at,
-                                      const Norm& n, int row, int rows_step) {
+  __device__ __forceinline__ NormWalk(const Norm& n, int group, int row, int rows_step) {
     const int b = row / n.L;
     L = n.L, t = row - b * L;
-    const T* q = (const T*)base + at;
-    last = q + (n.batch - 1) * sb + (L - 1) * st;
-    p = q + b * sb + t * st;
     step_t = rows_step % L;
-    step = rows_step / L * sb + step_t * st;
-    wrap = sb - L * st;
     left = n.batch * L - row;   // rows from this one to the end
+#pragma unroll
+    for (int k = 0; k < M; ++k) {
+      const long long sb = k ? n.z_b : n.x_b, st = k ? n.z_t : n.x_t, sg = k ? n.z_g : n.x_g;
+      const T* q = (const T*)(k ? n.gate : n.x) + group * sg;
+      last[k] = q + (n.batch - 1) * sb + (L - 1) * st;
+      p[k] = q + b * sb + t * st;
+      step[k] = rows_step / L * sb + step_t * st;
+      wrap[k] = sb - L * st;
+    }
   }
-  __device__ __forceinline__ const T* row() const { return left > 0 ? p : last; }
+  __device__ __forceinline__ const T* row(int k) const { return left > 0 ? p[k] : last[k]; }
   __device__ __forceinline__ void next(int rows_step) {
     left -= rows_step;
-    p += step;
     t += step_t;
-    if (t >= L) t -= L, p += wrap;
+    const bool over = t >= L;
+    if (over) t -= L;
+#pragma unroll
+    for (int k = 0; k < M; ++k) p[k] += over ? step[k] + wrap[k] : step[k];
   }
 };
-
-// f with whether there is a gate and an activation as constants
-template <class F>
-__device__ __forceinline__ void norm_forms(const Norm& p, F f) {
-  using std::false_type;
-  using std::true_type;
-  if (p.gate) {
-    if (p.act) f(true_type(), true_type());
-    else f(true_type(), false_type());
-  } else {
-    if (p.act) f(false_type(), true_type());
-    else f(false_type(), false_type());
-  }
-}
 
 template <typename T, NormFit FIT, int N>
 struct NormRow {
@@ -137,74 +134,86 @@ __device__ __forceinline__ void norm_params(const Norm& p, const NormPlace<FIT, 
 // mean and 1 / sqrt(var + eps) of a group's row
 template <typename T, NormFit FIT, int N>
 __device__ __forceinline__ void norm_stats(const NormRow<T, FIT, N>& x, const Norm& p,
-                                           const NormPlace<FIT, N>& at, float* red, float& mean,
+                                           const NormPlace<FIT, N>& at, float (&red)[1][4], float& mean,
                                            float& rstd) {
-  float sum = 0.f;
+  float sum[1] = {0.f};
 #pragma unroll
   for (int j = 0; j < N; ++j)
 #pragma unroll
-    for (int i = 0; i < 8; ++i) sum += at.has(j, i) ? x.v[j].r.at(i) : 0.f;
-  mean = group_sum(sum, p.tpg, red) * p.inv_w;
-  sum = 0.f;
+    for (int i = 0; i < 8; ++i) sum[0] += at.has(j, i) ? x.v[j].r.at(i) : 0.f;
+  group_sums(sum, p.tpg, red);
+  mean = sum[0] * p.inv_w;
+  sum[0] = 0.f;
 #pragma unroll
   for (int j = 0; j < N; ++j)
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
       const float d = at.has(j, i) ? x.v[j].r.at(i) - mean : 0.f;
-      sum = fmaf(d, d, sum);
+      sum[0] = fmaf(d, d, sum[0]);
     }
-  rstd = __builtin_amdgcn_rsqf(fmaf(group_sum(sum, p.tpg, red), p.inv_w, p.eps));   // within 1 ulp
+  group_sums(sum, p.tpg, red);
+  rstd = __builtin_amdgcn_rsqf(fmaf(sum[0], p.inv_w, p.eps));   // within 1 ulp
 }
 
-template <typename T, NormFit FIT, int N>
+template <typename T, NormFit FIT, int N, bool GATE, bool ACT>
 __global__ __launch_bounds__(NORM_THREADS) void norm_fwd_kernel(Norm p) {
-  __shared__ float red[4];
+  __shared__ float red[1][4];
   const NormPlace<FIT, N> at(p);
   float w[N][8], bias[N][8];
   norm_params(p, at, w, bias);
   const int rows = p.batch * p.L, step = p.row_blocks * p.rb;
   int row = blockIdx.x * p.rb + at.slot;
-  NormRows<T> xr(p.x, p.x_b, p.x_t, at.group * p.x_g, p, row, step);
-  NormRows<T> zr(p.gate, p.z_b, p.z_t, at.group * p.z_g, p, row, step);
-  NormRow<T, FIT, N> x, z;
-  auto load = [&] {
-    x.load(xr.row(), p, at.first);
-    if (p.gate) z.load(zr.row(), p, at.first);
-    xr.next(step);
-    if (p.gate) zr.next(step);
+  NormWalk<T, GATE> walk(p, at.group, row, step);
+  struct Rows {
+    NormRow<T, FIT, N> x, z;
   };
-  load();
+  auto load = [&](Rows& r) {
+    r.x.load(walk.row(0), p, at.first);
+    if constexpr (GATE) r.z.load(walk.row(1), p, at.first);
+    walk.next(step);
+  };
   T* y = (T*)p.y + ((long long)row * p.G + at.group) * p.W;
   const long long y_step = (long long)step * p.G * p.W;
-  // every thread makes the same number of rounds: group_sum may hold a barrier
-  for (int first = blockIdx.x * p.rb; first < rows; first += step, row += step, y += y_step) {
-    const NormRow<T, FIT, N> cx = x, cz = z;
-    if (first + step < rows) load();
+  auto work = [&](const Rows& r) {
     float mean, rstd;
-    norm_stats(cx, p, at, red, mean, rstd);
-    if (!at.in || row >= rows) continue;
-    norm_forms(p, [&](auto gate, auto act) {
+    norm_stats(r.x, p, at, red, mean, rstd);
+    if (!at.in || row >= rows) return;
 #pragma unroll
-      for (int j = 0; j < N; ++j) {
-        Cols<T, NormRow<T, FIT, N>::VEC, 8> out;
+    for (int j = 0; j < N; ++j) {
+      Cols<T, NormRow<T, FIT, N>::VEC, 8> out;
+      float os[8];
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          float o = fmaf((cx.v[j].r.at(i) - mean) * rstd, w[j][i], bias[j][i]);
-          const float a = gate.value ? cz.v[j].r.at(i) : o;
-          if (act.value) o *= gate.value ? a * sigmoid(a) : sigmoid(a);
-          else if (gate.value) o *= a;
-          out.r.set(i, o);
-        }
-        if (at.own[j]) out.store(y + at.first[j], p.W);
+      for (int i = 0; i < 8; ++i) {
+        float o = fmaf((r.x.v[j].r.at(i) - mean) * rstd, w[j][i], bias[j][i]);
+        const float a = GATE ? r.z.v[j].r.at(i) : o;
+        if (ACT) o *= GATE ? a * sigmoid(a) : sigmoid(a);
+        else if (GATE) o *= a;
+        os[i] = o;
       }
-    });
+      out.r.pack(os);
+      if (at.own[j]) out.store(y + at.first[j], p.W);
+    }
+  };
+  // Two rows by turns, one on its way while the other is worked on; every thread makes the
+  // same number of rounds, as a group's sums may hold a barrier
+  Rows even, odd;
+  load(even);
+  int first = blockIdx.x * p.rb;
+  auto round = [&](const Rows& now, Rows& next) {
+    const bool more = first + step < rows;
+    if (more) load(next);
+    work(now);
+    first += step, row += step, y += y_step;
+    return more;
+  };
+  while (round(even, odd) && round(odd, even)) {
   }
 }
 
-template <typename T, NormFit FIT, int N>
-__global__ __launch_bounds__(NORM_THREADS, N == 1 ? 4 : 1) void norm_bwd_kernel(Norm p, const void* dy_, void* dx_,
-                                                                void* dgate_, float* part) {
-  __shared__ float red[4];
+template <typename T, NormFit FIT, int N, bool GATE, bool ACT>
+__global__ __launch_bounds__(NORM_THREADS, N == 1 ? 4 : 1) void norm_bwd_kernel(
+    Norm p, const void* dy_, void* dx_, void* dgate_, float* part) {
+  __shared__ float red[1][4], red2[2][4];
   __shared__ float shares[NORM_THREADS][9];
   const NormPlace<FIT, N> at(p);
   constexpr bool VEC = NormRow<T, FIT, N>::VEC;
@@ -216,73 +225,84 @@ __global__ __launch_bounds__(NORM_THREADS, N == 1 ? 4 : 1) void norm_bwd_kernel(
     for (int i = 0; i < 8; ++i) dw[j][i] = db[j][i] = 0.f;
   const int rows = p.batch * p.L, step = p.row_blocks * p.rb;
   int row = blockIdx.x * p.rb + at.slot;
-  NormRows<T> xr(p.x, p.x_b, p.x_t, at.group * p.x_g, p, row, step);
-  NormRows<T> zr(p.gate, p.z_b, p.z_t, at.group * p.z_g, p, row, step);
+  NormWalk<T, GATE> walk(p, at.group, row, step);
   long long out = ((long long)row * p.G + at.group) * p.W;   // of dy, dx, dgate
   const long long out_step = (long long)step * p.G * p.W;
   const long long out_last = ((long long)(rows - 1) * p.G + at.group) * p.W;
-  NormRow<T, FIT, N> x, z, g;
-  auto load = [&](long long o) {
-    x.load(xr.row(), p, at.first);
-    if (p.gate) z.load(zr.row(), p, at.first);
-    g.load((const T*)dy_ + min(o, out_last), p, at.first);
-    xr.next(step);
-    if (p.gate) zr.next(step);
+  struct Rows {
+    NormRow<T, FIT, N> x, z, g;
   };
-  load(out);
-  for (int first = blockIdx.x * p.rb; first < rows; first += step, row += step, out += out_step) {
-    const NormRow<T, FIT, N> cx = x, cz = z, cg = g;
-    if (first + step < rows) load(out + out_step);
+  auto load = [&](Rows& r, long long o) {
+    r.x.load(walk.row(0), p, at.first);
+    if constexpr (GATE) r.z.load(walk.row(1), p, at.first);
+    r.g.load((const T*)dy_ + min(o, out_last), p, at.first);
+    walk.next(step);
+  };
+  auto work = [&](const Rows& r) {
     float mean, rstd;
-    norm_stats(cx, p, at, red, mean, rstd);
+    norm_stats(r.x, p, at, red, mean, rstd);
     const bool have = at.in && row < rows;
-    float s1 = 0.f, s2 = 0.f, dn[N][8];
-    norm_forms(p, [&](auto gate, auto act) {
+    float s[2] = {0.f, 0.f}, dn[N][8];   // of dn and of dn n
 #pragma unroll
-      for (int j = 0; j < N; ++j) {
-        Cols<T, VEC, 8> dz;
+    for (int j = 0; j < N; ++j) {
+      Cols<T, VEC, 8> dz;
+      float dzs[8];
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          const float n = (cx.v[j].r.at(i) - mean) * rstd, o = fmaf(n, w[j][i], bias[j][i]);
-          const float dy = cg.v[j].r.at(i);
-          float d = dy;
-          if (gate.value) {
-            const float z1 = cz.v[j].r.at(i), s = sigmoid(z1);
-            d = dy * (act.value ? z1 * s : z1);
-            dz.r.set(i, dy * o * (act.value ? s * fmaf(z1, 1.f - s, 1.f) : 1.f));
-          } else if (act.value) {
-            const float s = sigmoid(o);
-            d = dy * (s * fmaf(o, 1.f - s, 1.f));
-          }
-          const float dn1 = d * w[j][i];
-          dn[j][i] = dn1;
-          if (FIT == FULL) {
-            s1 += dn1;
-            s2 = fmaf(dn1, n, s2);
-          } else {
-            s1 += at.has(j, i) ? dn1 : 0.f;
-            s2 += at.has(j, i) ? dn1 * n : 0.f;
-          }
-          d = have ? d : 0.f;   // a row past the last adds nothing
-          db[j][i] += d;
-          dw[j][i] = fmaf(d, n, dw[j][i]);
+      for (int i = 0; i < 8; ++i) {
+        const float n = (r.x.v[j].r.at(i) - mean) * rstd, o = fmaf(n, w[j][i], bias[j][i]);
+        const float dy = r.g.v[j].r.at(i);
+        float d = dy;
+        if (GATE) {
+          const float z1 = r.z.v[j].r.at(i), a = sigmoid(z1);
+          d = dy * (ACT ? z1 * a : z1);
+          dzs[i] = dy * o * (ACT ? a * fmaf(z1, 1.f - a, 1.f) : 1.f);
+        } else if (ACT) {
+          const float a = sigmoid(o);
+          d = dy * (a * fmaf(o, 1.f - a, 1.f));
         }
-        if (gate.value && have && at.own[j]) dz.store((T*)dgate_ + out + at.first[j], p.W);
+        const float dn1 = d * w[j][i];
+        dn[j][i] = dn1;
+        if (FIT == FULL) {
+          s[0] += dn1;
+          s[1] = fmaf(dn1, n, s[1]);
+        } else {
+          s[0] += at.has(j, i) ? dn1 : 0.f;
+          s[1] += at.has(j, i) ? dn1 * n : 0.f;
+        }
+        d = have ? d : 0.f;   // a row past the last adds nothing
+        db[j][i] += d;
+        dw[j][i] = fmaf(d, n, dw[j][i]);
       }
-    });
-    const float m1 = group_sum(s1, p.tpg, red) * p.inv_w;
-    const float m2 = group_sum(s2, p.tpg, red) * p.inv_w;
-    if (!have) continue;
+      if (GATE) dz.r.pack(dzs);
+      if (GATE && have && at.own[j]) dz.store((T*)dgate_ + out + at.first[j], p.W);
+    }
+    group_sums(s, p.tpg, red2);
+    if (!have) return;
+    const float m1 = s[0] * p.inv_w, m2 = s[1] * p.inv_w;
 #pragma unroll
     for (int j = 0; j < N; ++j) {
       Cols<T, VEC, 8> dx;
+      float dxs[8];
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
-        const float n = (cx.v[j].r.at(i) - mean) * rstd;
-        dx.r.set(i, rstd * (dn[j][i] - fmaf(n, m2, m1)));
+        const float n = (r.x.v[j].r.at(i) - mean) * rstd;
+        dxs[i] = rstd * (dn[j][i] - fmaf(n, m2, m1));
       }
+      dx.r.pack(dxs);
       if (at.own[j]) dx.store((T*)dx_ + out + at.first[j], p.W);
     }
+  };
+  Rows even, odd;
+  load(even, out);
+  int first = blockIdx.x * p.rb;
+  auto round = [&](const Rows& now, Rows& next) {   // as in the forward
+    const bool more = first + step < rows;
+    if (more) load(next, out + out_step);
+    work(now);
+    first += step, row += step, out += out_step;
+    return more;
+  };
+  while (round(even, odd) && round(odd, even)) {
   }
   if (!part) return;
   // the rb rows' shares of each channel, in order: part [row blocks][2][G W]
@@ -330,28 +350,60 @@ void norm_split(Norm& p, bool backward) {
   p.row_blocks = (int)(rows < blocks ? rows : blocks);
 }
 
-#define LZ_NORM_VECS(T, FIT, KERN, ...)                                                        \
-  if (p.vecs == 1) hipLaunchKernelGGL((KERN<T, FIT, 1>), grid, block, 0, st, __VA_ARGS__);      \
-  else if (p.vecs == 2) hipLaunchKernelGGL((KERN<T, FIT, 2>), grid, block, 0, st, __VA_ARGS__); \
-  else hipLaunchKernelGGL((KERN<T, FIT, 4>), grid, block, 0, st, __VA_ARGS__)
-#define LZ_NORM_FITS(T, KERN, ...)                                                             \
-  if (p.W < 8) hipLaunchKernelGGL((KERN<T, NARROW, 1>), grid, block, 0, st, __VA_ARGS__);       \
-  else if (p.W == 8 * p.tpg * (p.vecs > 2 ? 4 : p.vecs)) { LZ_NORM_VECS(T, FULL, KERN, __VA_ARGS__); } \
-  else { LZ_NORM_VECS(T, TAIL, KERN, __VA_ARGS__); }
-#define LZ_NORM_TYPES(KERN, ...)                  \
-  if (is_bf16) { LZ_NORM_FITS(bf16, KERN, __VA_ARGS__) } \
-  else { LZ_NORM_FITS(float, KERN, __VA_ARGS__) }
+template <typename T, NormFit FIT_, int N_>
+struct NormForm {
+  using type = T;
+  static constexpr NormFit FIT = FIT_;
+  static constexpr int N = N_;
+};
+// Calls f with the template arguments that p and the type ask for
+template <typename T, NormFit FIT, int N, class F>
+void norm_forms(const Norm& p, F f) {
+  using A = NormForm<T, FIT, N>;
+  if (p.gate) {
+    if (p.act) f(A(), std::true_type(), std::true_type());
+    else f(A(), std::true_type(), std::false_type());
+  } else {
+    if (p.act) f(A(), std::false_type(), std::true_type());
+    else f(A(), std::false_type(), std::false_type());
+  }
+}
+template <typename T, NormFit FIT, class F>
+void norm_vecs(const Norm& p, F f) {
+  if (p.vecs == 1) norm_forms<T, FIT, 1>(p, f);
+  else if (p.vecs == 2) norm_forms<T, FIT, 2>(p, f);
+  else norm_forms<T, FIT, 4>(p, f);
+}
+template <typename T, class F>
+void norm_fits(const Norm& p, F f) {
+  if (p.W < 8) norm_forms<T, NARROW, 1>(p, f);
+  else if (p.W == 8 * p.tpg * (p.vecs > 2 ? 4 : p.vecs)) norm_vecs<T, FULL>(p, f);
+  else norm_vecs<T, TAIL>(p, f);
+}
+template <class F>
+void norm_types(const Norm& p, bool is_bf16, F f) {
+  if (is_bf16) norm_fits<bf16>(p, f);
+  else norm_fits<float>(p, f);
+}
 
 hipError_t launch_norm_fwd(const Norm& p, bool is_bf16, hipStream_t st) {
   const dim3 grid(p.row_blocks, p.group_blocks), block(NORM_THREADS);
-  LZ_NORM_TYPES(norm_fwd_kernel, p)
+  norm_types(p, is_bf16, [&](auto form, auto gate, auto act) {
+    using A = decltype(form);
+    hipLaunchKernelGGL((norm_fwd_kernel<typename A::type, A::FIT, A::N, gate.value, act.value>), grid,
+                       block, 0, st, p);
+  });
   return hipGetLastError();
 }
 
 hipError_t launch_norm_bwd(const Norm& p, const void* dy, void* dx, void* dgate, float* part,
                            float* dw, float* dbias, bool is_bf16, hipStream_t st) {
   const dim3 grid(p.row_blocks, p.group_blocks), block(NORM_THREADS);
-  LZ_NORM_TYPES(norm_bwd_kernel, p, dy, dx, dgate, part)
+  norm_types(p, is_bf16, [&](auto form, auto gate, auto act) {
+    using A = decltype(form);
+    hipLaunchKernelGGL((norm_bwd_kernel<typename A::type, A::FIT, A::N, gate.value, act.value>), grid,
+                       block, 0, st, p, dy, dx, dgate, part);
+  });
   if (hipError_t e = hipGetLastError(); e != hipSuccess) return e;
   if (!part) return hipSuccess;
   const int C = p.G * p.W;

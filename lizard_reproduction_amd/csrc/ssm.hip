@@ -79,8 +79,7 @@ __global__ __launch_bounds__(64 * (W + H)) void ssm_fwd_kernel(Ssm p) {
     if (has_z) {
       if (p.mixed) {
         RawRow<float, V, VEC> m;
-#pragma unroll
-        for (int i = 0; i < V; ++i) m.set(i, y[i]);
+        m.pack(y);
         store_raw<float, V, VEC>(open_rsrc(p.mixed + ((long long)at.b * p.L + t0) * E + at.c0),
                                  row * E + tc, row < rows, left, m);
       }
@@ -95,8 +94,7 @@ __global__ __launch_bounds__(64 * (W + H)) void ssm_fwd_kernel(Ssm p) {
       for (int i = 0; i < V; ++i) y[i] = 0.f;
     }
     RawRow<T, V, VEC> out;
-#pragma unroll
-    for (int i = 0; i < V; ++i) out.set(i, y[i]);
+    out.pack(y);
     store_raw<T, V, VEC>(ry, row * E + tc, row < p.L - t0, left, out);
     yb += SSM_TT * (long long)E;
   };

@@ -174,25 +174,28 @@ __global__ __launch_bounds__(64 * (W + SSM_HELPERS), W == 8 ? 3 : 2) void ssm_bw
 #pragma unroll
       for (int j = 0; j < 2; ++j) {
         RawRow<float, V, VEC> r;
-#pragma unroll
-        for (int i = 0; i < V; ++i) r.set(i, sum[j][i]);
+        r.pack(sum[j]);
         store_raw<float, V, VEC>(open_rsrc(gr.acc + j * gr.acc_step + o), off, in, left, r);
       }
       return;
     }
     RawRow<T, V, VEC> ox, od, oz;
+    float dx[V], ddts[V];
 #pragma unroll
     for (int i = 0; i < V; ++i) {
       const float ddt = fmaf(k.x[i], sum[0][i], sum[1][i] * LN2) * k.slope[i];
-      ox.set(i, fmaf(k.delta[i], sum[0][i], D[i] * k.dm[i]));
-      od.set(i, ddt);
-      if (has_z) oz.set(i, k.dz[i]);
+      dx[i] = fmaf(k.delta[i], sum[0][i], D[i] * k.dm[i]);
+      ddts[i] = ddt;
       dD[i] = fmaf(k.dm[i], k.x[i], dD[i]);   // x and dy are zero where there is no row
       if (in && i < left) dbias[i] += ddt;
     }
+    ox.pack(dx), od.pack(ddts);
     store_raw<T, V, VEC>(open_rsrc((T*)gr.dx + o), off, in, left, ox);
     store_raw<T, V, VEC>(open_rsrc((T*)gr.ddt + o), off, in, left, od);
-    if (has_z) store_raw<T, V, VEC>(open_rsrc((T*)gr.dz + o), off, in, left, oz);
+    if (has_z) {
+      oz.pack(k.dz);
+      store_raw<T, V, VEC>(open_rsrc((T*)gr.dz + o), off, in, left, oz);
+    }
   };
 
   // --- the walk (scan) --------------------------------------------------------------------
