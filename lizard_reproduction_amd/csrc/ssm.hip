@@ -12,7 +12,7 @@
 namespace lz {
 
 // STATE: the segments' own states alone, without C, z and y.
-template <typename T, int W, int NP, int H, bool VEC, bool STATE>
+template <typename T, int W, int NP, int NS, int H, bool VEC, bool STATE>
 __global__ __launch_bounds__(64 * (W + H)) void ssm_fwd_kernel(Ssm p) {
   constexpr int V = SSM_TILE / (64 * H), COLS = SSM_CH / V;
   // two tiles of each: one worked on by the scan waves, one by the helpers
@@ -106,14 +106,14 @@ __global__ __launch_bounds__(64 * (W + H)) void ssm_fwd_kernel(Ssm p) {
   const T* Bb = (const T*)p.B + at.b * p.B_b + first * B_t + (long long)at.g * p.B_g;
   const T* Cb = (const T*)p.C + at.b * p.C_b + first * C_t + (long long)at.g * p.C_g;
   float* saved = p.saved ? p.saved + ((size_t)at.b * p.tiles + at.tile0) * N * E : nullptr;
-  float A2[NP][4], h[NP][4], dsum = 0.f;
-  SsmVec<T, 4> Bv[NP], Cv[NP];
+  float A2[NP][NS], h[NP][NS], dsum = 0.f;
+  SsmVec<T, NS> Bv[NP], Cv[NP];
   auto start = [&] {
 #pragma unroll
     for (int q = 0; q < NP; ++q)
 #pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        const int n = 4 * (w + W * q) + k;
+      for (int k = 0; k < NS; ++k) {
+        const int n = NS * (w + W * q) + k;
         const bool in = mine && n < N;
         A2[q][k] = in ? p.A[(size_t)c * N + n] * LOG2E : 0.f;
         h[q][k] = in && !STATE && p.state_in ? p.state_in[((size_t)at.b * E + c) * N + n] : 0.f;
@@ -126,8 +126,8 @@ __global__ __launch_bounds__(64 * (W + H)) void ssm_fwd_kernel(Ssm p) {
 #pragma unroll
         for (int q = 0; q < NP; ++q)
 #pragma unroll
-          for (int k = 0; k < 4; ++k) {
-            const int n = 4 * (w + W * q) + k;
+          for (int k = 0; k < NS; ++k) {
+            const int n = NS * (w + W * q) + k;
             if (mine && n < N)
               h[q][k] = fmaf(__builtin_amdgcn_exp2f(A2[q][k] * d), h[q][k],
                              p.rec[(rec * N + n) * E + c]);
@@ -138,18 +138,18 @@ __global__ __launch_bounds__(64 * (W + H)) void ssm_fwd_kernel(Ssm p) {
   auto load_bc = [&](int rows) {
 #pragma unroll
     for (int q = 0; q < NP; ++q) {
-      Bv[q].load(Bb, rows, B_t, N, 4 * (w + W * q), lane);
-      if (!STATE) Cv[q].load(Cb, rows, C_t, N, 4 * (w + W * q), lane);
+      Bv[q].load(Bb, rows, B_t, N, NS * (w + W * q), lane);
+      if (!STATE) Cv[q].load(Cb, rows, C_t, N, NS * (w + W * q), lane);
     }
     Bb += SSM_TT * (long long)B_t;
     Cb += SSM_TT * (long long)C_t;
   };
-  float Bf[NP][4], Cf[NP][4];
+  float Bf[NP][NS], Cf[NP][NS];
   auto take_bc = [&] {
 #pragma unroll
     for (int q = 0; q < NP; ++q)
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
+      for (int i = 0; i < NS; ++i) {
         Bf[q][i] = Bv[q].at(i);
         if (!STATE) Cf[q][i] = Cv[q].at(i);
       }
@@ -159,34 +159,40 @@ __global__ __launch_bounds__(64 * (W + H)) void ssm_fwd_kernel(Ssm p) {
 #pragma unroll
     for (int q = 0; q < NP; ++q)
 #pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        const int n = 4 * (w + W * q) + k;
+      for (int k = 0; k < NS; ++k) {
+        const int n = NS * (w + W * q) + k;
         if (mine && n < N) saved[(size_t)n * E + c] = h[q][k];
       }
     saved += (size_t)N * E;
   };
   auto scan = [&](int buf) {
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const f32x4 dl = get_tokens(sd[buf], 4 * i, lane), ul = get_tokens(su[buf], 4 * i, lane);
+    constexpr int TOKENS = SsmVec<T, NS>::TOKENS;
+    f32x4 dn = get_tokens(sd[buf], 0, lane), un = get_tokens(su[buf], 0, lane);
+    static_for<4>([&](auto ki) {
+      constexpr int i = decltype(ki)::value;
+      const f32x4 dl = dn, ul = un;
+      if (i < 3) dn = get_tokens(sd[buf], 4 * i + 4, lane), un = get_tokens(su[buf], 4 * i + 4, lane);
+      __builtin_amdgcn_sched_barrier(0);   // the next four tokens' reads go out before these are used
       f32x4 yl = {0.f, 0.f, 0.f, 0.f};
       if (STATE) dsum += (dl[0] + dl[1]) + (dl[2] + dl[3]);
 #pragma unroll
       for (int q = 0; q < NP; ++q) {
-        float hs[4][4];
+        float hs[4][NS];
         static_for<4>([&](auto kt) {
-          constexpr int t = decltype(kt)::value;
-          static_for<4>([&](auto kn) {
+          constexpr int t = decltype(kt)::value, at_t = (4 * i + t) % TOKENS;
+          static_for<NS>([&](auto kn) {
             constexpr int n = decltype(kn)::value;
             const float a = __builtin_amdgcn_exp2f(dl[t] * A2[q][n]);
-            h[q][n] = fmaf(a, h[q][n], dpp<DPP_BCAST + 4 * t + n>(Bf[q][i]) * ul[t]);
+            h[q][n] = fmaf(a, h[q][n],
+                           dpp<DPP_BCAST + NS * at_t + n>(Bf[q][4 * i / TOKENS]) * ul[t]);
             hs[t][n] = h[q][n];
           });
         });
-        if (!STATE) ssm_dots4(yl, Cf[q][i], hs);
+        if constexpr (!STATE && NS == 4) ssm_dots4(yl, Cf[q][i], hs);
+        if constexpr (!STATE && NS == 2) ssm_dots<8 * (i & 1)>(yl, Cf[q][i >> 1], hs);
       }
       if (!STATE) put_tokens(sy[STATE ? 0 : buf * W + w], 4 * i, lane, yl);
-    }
+    });
   };
   auto end = [&] {
     if (!mine) return;
@@ -195,8 +201,8 @@ __global__ __launch_bounds__(64 * (W + H)) void ssm_fwd_kernel(Ssm p) {
 #pragma unroll
     for (int q = 0; q < NP; ++q)
 #pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        const int n = 4 * (w + W * q) + k;
+      for (int k = 0; k < NS; ++k) {
+        const int n = NS * (w + W * q) + k;
         if (n >= N) continue;
         if (STATE)
           p.rec[(rec * N + n) * E + c] = h[q][k];
@@ -206,6 +212,7 @@ __global__ __launch_bounds__(64 * (W + H)) void ssm_fwd_kernel(Ssm p) {
   };
 
   const int t0 = at.tile0, t1 = at.tile1;   // t0 < t1
+  if (wave < W) __builtin_amdgcn_s_setprio(2);   // the scan is the longer of the two
   if (wave >= W) {
     // the rows of two tiles ahead on their way, of this tile and the one before kept to
     // their end; a tile's sums go out after the next rows have come, so that nothing waits
@@ -309,30 +316,33 @@ __global__ __launch_bounds__(256) void ssm_step_kernel(Ssm p, float* state) {
   }
 }
 
-template <typename T, int W, int NP, bool VEC>
+template <typename T, int W, int NP, int NS, int H, bool VEC>
 hipError_t fwd_launch(const Ssm& p, hipStream_t st) {
   const int nblk = p.G * p.gblocks;
-  constexpr int H = SSM_FWD_HELPERS;
   const dim3 block(64 * (W + H));
   if (p.S > 1) {
-    hipLaunchKernelGGL((ssm_fwd_kernel<T, W, NP, H, VEC, true>), dim3(nblk * (p.S - 1) * p.batch),
-                       block, 0, st, p);
+    hipLaunchKernelGGL((ssm_fwd_kernel<T, W, NP, NS, H, VEC, true>),
+                       dim3(nblk * (p.S - 1) * p.batch), block, 0, st, p);
     if (hipError_t e = hipGetLastError(); e != hipSuccess) return e;
   }
-  hipLaunchKernelGGL((ssm_fwd_kernel<T, W, NP, H, VEC, false>), dim3(nblk * p.S * p.batch), block,
-                     0, st, p);
+  hipLaunchKernelGGL((ssm_fwd_kernel<T, W, NP, NS, H, VEC, false>), dim3(nblk * p.S * p.batch),
+                     block, 0, st, p);
   return hipGetLastError();
 }
 
+// Scan waves W of NS states (and NP passes of them) and helper waves H for N states.  Up to
+// eight states a wave takes two, as one wave a SIMD, the channels few or many, is bound by
+// its own latency (N = 8, 4096 tokens x 4096 channels: 87 us, with four a wave 124; N = 16,
+// eight waves of two against four of four, whose sums and reads of LDS are half as many: 129
+// against 125).  Eight scan waves leave room for four helpers where eight would do (N = 32:
+// 202 against 214 us; with four scan waves, N = 16, training: 562 with four, 551 with eight).
 template <typename T, bool VEC>
 hipError_t fwd_waves(const Ssm& p, hipStream_t st) {
-  const SsmWaves n = ssm_fwd_waves(p.N);
-  switch (n.W) {
-    case 1: return fwd_launch<T, 1, 1, VEC>(p, st);
-    case 2: return fwd_launch<T, 2, 1, VEC>(p, st);
-    case 4: return fwd_launch<T, 4, 1, VEC>(p, st);
-    default: return n.NP == 1 ? fwd_launch<T, 8, 1, VEC>(p, st) : fwd_launch<T, 8, 2, VEC>(p, st);
-  }
+  if (p.N <= 4) return fwd_launch<T, 2, 1, 2, 8, VEC>(p, st);
+  if (p.N <= 8) return fwd_launch<T, 4, 1, 2, 8, VEC>(p, st);
+  if (p.N <= 16) return fwd_launch<T, 4, 1, 4, 8, VEC>(p, st);
+  if (p.N <= 32) return fwd_launch<T, 8, 1, 4, 4, VEC>(p, st);
+  return fwd_launch<T, 8, 2, 4, 4, VEC>(p, st);
 }
 
 // Segments of a sequence.  One where the 64-channel blocks fill the chip, as a pass over

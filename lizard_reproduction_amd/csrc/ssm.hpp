@@ -9,12 +9,12 @@ namespace lz {
 
 // Layout of the work.  A workgroup takes 64 channels of one group and one sequence (or a
 // segment of it) and walks it in tiles of 16 tokens.  In its W scan waves a lane is a
-// channel; wave w holds NS states in registers, four in the forward (and another four from
-// 4 (w + W) on with NP = 2), two in the backward.  Four helper waves turn the next tile's rows into delta, u and
-// the like while the scan waves walk this one, and the last tile's sums into rows: one
-// barrier a tile, and waves to switch between though a wave holds 256 states.  (With the
-// scan waves doing both, two barriers a tile, the training pass of 8192 tokens x 4096
-// channels x 16 states took 857 us where this takes 738.)
+// channel; a wave holds NS states in registers, two or four (and another NS from NS (w + W)
+// on with NP = 2) in the forward, two in the backward.  Helper waves turn the next tile's
+// rows into delta, u and the like while the scan waves walk this one, and the last tile's
+// sums into rows: one barrier a tile, and other waves to switch to while one waits.  (With
+// the scan waves doing both, two barriers a tile, the training pass of 8192 tokens x 4096
+// channels x 16 states took 857 us where this took 738.)
 // In LDS a tile is rows of the 64 channels: a thread's share of a row is one vector, a
 // wave's read of a token 64 consecutive floats (channels of 16 tokens each, 20 floats
 // apart, made the transposed writes and reads conflict: 40 % of the forward's time).
@@ -54,10 +54,10 @@ struct SsmGrad {
   int NQ;                // padded states in part_bc
 };
 
-// Helper waves of a workgroup: eight in the forward (four: training 8192 tokens x 4096
-// channels 267 against 254 us), four in the backward, whose registers leave room for twelve
-// waves.  A thread of theirs takes a vector of V channels of one row of a tile.
-constexpr int SSM_FWD_HELPERS = 8, SSM_HELPERS = 4, SSM_V = SSM_TILE / (64 * SSM_HELPERS);
+// Helper waves of the backward (the forward's are chosen with its scan waves): its registers
+// leave room for twelve waves.  A thread of theirs takes a vector of V channels of one row of
+// a tile.
+constexpr int SSM_HELPERS = 4, SSM_V = SSM_TILE / (64 * SSM_HELPERS);
 constexpr int SSM_COLS = SSM_CH / SSM_V, SSM_ROWS = 64 * SSM_HELPERS / SSM_COLS;
 static_assert(SSM_V == 4 && SSM_ROWS == SSM_TT, "a thread, a vector of the tile");
 
@@ -189,14 +189,6 @@ struct SsmPlace {
   }
 };
 
-// Scan waves W and passes NP of the forward for N states
-struct SsmWaves {
-  int W, NP;
-};
-inline SsmWaves ssm_fwd_waves(int N) {
-  return N <= 4 ? SsmWaves{1, 1} : N <= 8 ? SsmWaves{2, 1} : N <= 16 ? SsmWaves{4, 1}
-       : N <= 32 ? SsmWaves{8, 1} : SsmWaves{8, 2};
-}
 // States the backward takes a launch, and N padded to whole launches
 constexpr int SSM_BWD_STATES = 16;
 inline int ssm_bwd_padded(int N) {
