@@ -3,10 +3,12 @@
 //   pre_t = bias + sum_{j < K} w_j x_{t-K+1+j},   y_t = pre_t or silu(pre_t)
 //
 // K is at most four, so a value takes a few operations and the bytes of x and y (backward:
-// x, dy, y's recomputation and dx) bound it.  A thread takes a vector of channels and a
-// run of tokens, with the K rows in registers: a row is read once by the run it lies in and again,
-// from cache, by the run after it.  A workgroup's threads are columns of vectors
-// times runs, a row's columns next to each other.
+// x, dy and dx) bound it.  A thread takes a vector of channels and a run of tokens, with the
+// K rows in registers: a row is read once by the run it lies in, and its last K - 1 again,
+// from cache, by the run after it.  A workgroup's threads are columns of vectors times runs,
+// a row's columns next to each other.  bf16, K = 4, 8192 tokens x 4096 channels: the forward
+// takes 28.7 us, 134 MB at 4.7 TB/s, the backward 45 us, 201 MB at 4.5 TB/s, where a copy
+// runs at 4.9; the last launch, which adds the runs' shares of dw and dbias, 4 us.
 //
 // Backward: g_t = dy_t act'(pre_t), dx_t = sum_j w_j g_{t+K-1-j} (the run goes K - 1 tokens
 // on), dw_j = sum_t g_t x_{t-K+1+j}, dbias = sum_t g_t: the workgroup's runs meet in LDS and
@@ -73,7 +75,7 @@ __device__ __forceinline__ void row_before(const Conv& p, const T* xb, int b, in
   for (int i = 0; i < V; ++i) v[i] = have ? c.r.at(i) : 0.f;
 }
 
-constexpr int CONV_AHEAD = 4;   // rows loaded before the first of them is used
+constexpr int CONV_AHEAD = 4;   // rows on their way while as many are worked on
 
 template <typename T, bool VEC, int K>
 __global__ __launch_bounds__(CONV_THREADS) void conv_fwd_kernel(Conv p) {
@@ -133,7 +135,8 @@ __global__ __launch_bounds__(CONV_THREADS) void conv_fwd_kernel(Conv p) {
   }
 }
 
-// One token of each sequence: a thread a channel, its kept rows moved up in place
+// One token of each sequence: a thread a channel, its kept rows moved up in place.  One
+// round of loads and the launch bound it (2.6 us at one sequence of 2048 channels).
 template <typename T, int K>
 __global__ __launch_bounds__(256) void conv_step_kernel(Conv p) {
   const int c = blockIdx.x * 256 + threadIdx.x, b = blockIdx.y;
@@ -258,12 +261,15 @@ __global__ __launch_bounds__(CONV_THREADS) void conv_bwd_kernel(Conv p, const vo
 }
 
 // Runs long enough that their K - 1 rows before them cost little, short enough that the
-// threads fill the chip twice over
+// threads fill the chip twice over.  (Threads a CU, training 8192 tokens x 4096 channels and
+// a forward of 5 x 1021 x 2050: 256 took 82 and 27 us, 512 81 and 15, 1024 85 and 15; runs of
+// at most 32, 64 and 128 tokens 82, 81 and 83 us of the first.)
 void conv_split(Conv& p, bool backward) {
   const int V = backward ? CONV_BWD_V : CONV_FWD_V, vecs = (p.C + V - 1) / V;
   int cols = 1;
   while (cols < 64 && cols < vecs) cols *= 2;
-  // fewer where the last block of columns would be mostly empty
+  // fewer where the last block of columns would be mostly empty (2050 channels: 15 us, with
+  // 64 columns all the same 23)
   while (cols > 16 && (vecs + cols - 1) / cols * cols * 8 > vecs * 9) cols /= 2;
   p.cols = cols;
   p.col_blocks = (vecs + cols - 1) / cols;

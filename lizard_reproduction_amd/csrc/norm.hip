@@ -5,9 +5,11 @@
 //
 // A group is read once into the registers of as many threads as it has vectors of eight
 // channels, its mean and then its squared distances from it summed across them in fp32, so
-// the rows' bytes bound it.  A thread keeps its channels, with w and b (backward: the sums
-// of dw and db) in registers, and goes through rows; the next row's loads are issued before
-// this row is worked on.  Groups may lie apart by any stride (the heads of an attention
+// the rows' bytes bound it (bf16, 8192 tokens of 32 groups of 128, with a gate: the forward
+// takes 43 us, 201 MB at 4.7 TB/s, the backward 65 us, 335 MB at 5.1 TB/s, where a copy runs at
+// 4.9).  A thread keeps its channels, with w and b (backward: the sums of dw and db) in
+// registers, and goes through rows; the next row's loads are issued before this row is
+// worked on.  Groups may lie apart by any stride (the heads of an attention
 // output); y is rows.
 //
 // Backward, from x again: do = dy act', dn = do w, dx = (dn - mean(dn) - n mean(dn n)) rstd,
@@ -155,6 +157,8 @@ __device__ __forceinline__ void norm_stats(const NormRow<T, FIT, N>& x, const No
   rstd = __builtin_amdgcn_rsqf(fmaf(sum[0], p.inv_w, p.eps));   // within 1 ulp
 }
 
+// The gate and the activation are template arguments: as branches in the loops over elements
+// they took the backward's walk 84 us where it now takes 65.
 template <typename T, NormFit FIT, int N, bool GATE, bool ACT>
 __global__ __launch_bounds__(NORM_THREADS) void norm_fwd_kernel(Norm p) {
   __shared__ float red[1][4];
@@ -330,8 +334,10 @@ __global__ __launch_bounds__(NORM_THREADS, N == 1 ? 4 : 1) void norm_bwd_kernel(
 }
 
 // Threads a group: a vector each, up to the workgroup; groups side by side, then rows.
-// The rows' blocks bring the forward to eight workgroups a CU (rows in flight hide the two
-// sums' latency) and the backward, whose blocks each write a share of dw and db, to four.
+// The rows' blocks bring the forward to eight workgroups a CU (3063 tokens of 32 groups of
+// 64: 9.8 us; with 4 and 16 a CU 10.3 and 10.6) and the backward, whose blocks each write a
+// share of dw and db, to four (8192 tokens of 32 groups of 128, with the shares' sums: 68 us
+// with 2 and 4, 84 with 8).
 void norm_split(Norm& p, bool backward) {
   const int vecs = (p.W + 7) / 8;
   int tpg = 1;

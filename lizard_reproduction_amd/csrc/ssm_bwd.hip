@@ -11,10 +11,16 @@
 // as in the forward and walks the tiles from the last; in each it walks forward once, every
 // decay and state of its 16 tokens staying in registers, then back.  What is
 // summed over n meets in LDS, the waves' shares side by side; what is summed over channels
-// is added across the wave, four tokens' sixteen sums at a time, and its 64-channel shares, as the sequences' shares
-// of dA, dD and dbias, go to memory for a second launch that adds them in
-// order: no atomics, the same bits every time.  More than 16 states are taken 16 a launch
+// is added across the wave, four tokens' sixteen sums at a time, and its 64-channel shares, as
+// the sequences' shares of dA, dD and dbias, go to memory for a second launch that adds them
+// in order: no atomics, the same bits every time.  More than 16 states are taken 16 a launch
 // (in one, a wave's registers did not hold them: N = 24 took 2.8 times as long as 16).
+//
+// The vector units bound it: B = 4, L = 2048, E = 4096, N = 16 in bf16 takes 435 us, 94 % of
+// them busy, a little over half with the twelve instructions and the exponential that each
+// (token, channel, n) takes.  (The sums over channels on the matrix units, 16 x 16 x 4 in
+// fp32: 470 -> 678 us, as their operands have to be laid out across lanes.  A helper's rows
+// kept by turns instead of copied: 3 % slower.)
 #include "ssm.hpp"
 
 namespace lz {

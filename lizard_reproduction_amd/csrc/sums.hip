@@ -3,7 +3,9 @@
 //
 // A workgroup takes 64 outputs, a lane each, its waves a run of the parts each; the
 // waves' sums meet in LDS and are added in wave order.  Consecutive lanes read
-// consecutive floats, so a job is as long as its partial results' bytes take.
+// consecutive floats, so a job is as long as its partial results' bytes take (the scan's dB
+// and dC of 8192 tokens x 16 states from 64 blocks of channels, 67 MB: 24 us with dA, dD and
+// dbias).
 #include "mixer_common.hpp"
 
 namespace lz {
