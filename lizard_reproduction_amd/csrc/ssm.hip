@@ -176,10 +176,10 @@ __global__ __launch_bounds__(64 * (W + H)) void ssm_fwd_kernel(Ssm p) {
       const f32x4 dl = dn, ul = un;
       if (i < 3) dn = get_tokens(sd[buf], 4 * i + 4, lane), un = get_tokens(su[buf], 4 * i + 4, lane);
       __builtin_amdgcn_sched_barrier(0);   // the next four tokens' reads go out before these are used
-      f32x4 yl = {0.f, 0.f, 0.f, 0.f};
+      f32x4 yl;
       if (STATE) dsum += (dl[0] + dl[1]) + (dl[2] + dl[3]);
-#pragma unroll
-      for (int q = 0; q < NP; ++q) {
+      static_for<NP>([&](auto kq) {
+        constexpr int q = decltype(kq)::value;
         float hs[4][NS];
         static_for<4>([&](auto kt) {
           constexpr int t = decltype(kt)::value, at_t = (4 * i + t) % TOKENS;
@@ -191,9 +191,8 @@ __global__ __launch_bounds__(64 * (W + H)) void ssm_fwd_kernel(Ssm p) {
             hs[t][n] = h[q][n];
           });
         });
-        if constexpr (!STATE && NS == 4) ssm_dots4(yl, Cf[q][i], hs);
-        if constexpr (!STATE && NS == 2) ssm_dots<8 * (i & 1)>(yl, Cf[q][i >> 1], hs);
-      }
+        if constexpr (!STATE) ssm_dots<4 * NS * i % 16, (q > 0)>(yl, Cf[q][4 * i / TOKENS], hs);
+      });
       if (!STATE) put_tokens(sy[STATE ? 0 : buf * W + w], 4 * i, lane, yl);
     });
   };

@@ -1,6 +1,7 @@
 // Arguments of the selective state space scan's kernels (ssm.hip, ssm_bwd.hip) and the
 // walk over a tile that both directions begin with.
 #pragma once
+#include <type_traits>
 #include <utility>
 
 #include "mixer_common.hpp"
@@ -103,7 +104,7 @@ __device__ __forceinline__ void put_tokens(float* tile, int t, int lane, const f
 template <typename T, int NS>
 struct SsmVec {
   static constexpr int TOKENS = 16 / NS;   // a register
-  uint32_t w[NS];
+  std::conditional_t<IS_BF16<T>, uint16_t, uint32_t> w[NS];   // as loaded until they are used
   __device__ __forceinline__ void load(const T* base, int rows, int pitch, int N, int n0, int lane) {
     const rsrc_t r = open_rsrc(base);
     const int n = n0 + lane % NS;
@@ -116,45 +117,73 @@ struct SsmVec {
     }
   }
   __device__ __forceinline__ float at(int i) const {
-    return __builtin_bit_cast(float, IS_BF16<T> ? w[i] << 16 : w[i]);
+    return __builtin_bit_cast(float, IS_BF16<T> ? (uint32_t)w[i] << 16 : (uint32_t)w[i]);
   }
 };
 
-// y[t] += sum_n v(K + NS t + n) h[t][n] for four tokens t, v(k) lane k of a row of 16: the
-// compiler folds the broadcast into a product but not into a multiply-add, so these are
-// written out, behind the two wait states that a DPP operand asks for after its register
-// was written.
-#define LZ_DOT(t, k, n) \
-  "v_fmac_f32_dpp %" #t ", %4, %" #n " row_newbcast:%" #k " row_mask:0xf bank_mask:0xf\n"
-template <int K>
+// y[t] = sum_n v(K + NS t + n) h[t][n] (ADD: added to y[t]) for four tokens t, v(k) lane k of
+// a row of 16: the compiler folds the broadcast into a product but not into a multiply-add,
+// so these are written out, behind the two wait states that a DPP operand asks for after its
+// register was written.
+#define LZ_DPP(op, t, k, n) \
+  op " %" #t ", %4, %" #n " row_newbcast:%" #k " row_mask:0xf bank_mask:0xf\n"
+#define LZ_FIRST LZ_DPP("v_mul_f32_dpp", 0, 13, 5) LZ_DPP("v_mul_f32_dpp", 1, 15, 7) \
+  LZ_DPP("v_mul_f32_dpp", 2, 17, 9) LZ_DPP("v_mul_f32_dpp", 3, 19, 11)
+#define LZ_DOT(t, k, n) LZ_DPP("v_fmac_f32_dpp", t, k, n)
+#define LZ_FIRST_ADD LZ_DOT(0, 13, 5) LZ_DOT(1, 15, 7) LZ_DOT(2, 17, 9) LZ_DOT(3, 19, 11)
+#define LZ_REST LZ_DOT(0, 14, 6) LZ_DOT(1, 16, 8) LZ_DOT(2, 18, 10) LZ_DOT(3, 20, 12)
+#define LZ_INS                                                                                 \
+  "v"(v), "v"(h[0][0]), "v"(h[0][1]), "v"(h[1][0]), "v"(h[1][1]), "v"(h[2][0]), "v"(h[2][1]), \
+      "v"(h[3][0]), "v"(h[3][1]), "n"(K), "n"(K + 1), "n"(K + 2), "n"(K + 3), "n"(K + 4),     \
+      "n"(K + 5), "n"(K + 6), "n"(K + 7)
+template <int K, bool ADD>
 __device__ __forceinline__ void ssm_dots(f32x4& y, float v, const float (&h)[4][2]) {
-  float y0 = y[0], y1 = y[1], y2 = y[2], y3 = y[3];
-  asm("s_nop 1\n"
-      LZ_DOT(0, 13, 5) LZ_DOT(1, 15, 7) LZ_DOT(2, 17, 9) LZ_DOT(3, 19, 11)
-      LZ_DOT(0, 14, 6) LZ_DOT(1, 16, 8) LZ_DOT(2, 18, 10) LZ_DOT(3, 20, 12)
-      : "+&v"(y0), "+&v"(y1), "+&v"(y2), "+&v"(y3)
-      : "v"(v), "v"(h[0][0]), "v"(h[0][1]), "v"(h[1][0]), "v"(h[1][1]), "v"(h[2][0]), "v"(h[2][1]),
-        "v"(h[3][0]), "v"(h[3][1]), "n"(K), "n"(K + 1), "n"(K + 2), "n"(K + 3), "n"(K + 4),
-        "n"(K + 5), "n"(K + 6), "n"(K + 7));
+  float y0, y1, y2, y3;
+  if constexpr (ADD) {
+    y0 = y[0], y1 = y[1], y2 = y[2], y3 = y[3];
+    asm("s_nop 1\n" LZ_FIRST_ADD LZ_REST : "+&v"(y0), "+&v"(y1), "+&v"(y2), "+&v"(y3) : LZ_INS);
+  } else {
+    asm("s_nop 1\n" LZ_FIRST LZ_REST : "=&v"(y0), "=&v"(y1), "=&v"(y2), "=&v"(y3) : LZ_INS);
+  }
   y = f32x4{y0, y1, y2, y3};
 }
-__device__ __forceinline__ void ssm_dots4(f32x4& y, float v, const float (&h)[4][4]) {
-  float y0 = y[0], y1 = y[1], y2 = y[2], y3 = y[3];
-#define LZ_DOT4(t, k, n) \
-  "v_fmac_f32_dpp %" #t ", %4, %" #n " row_newbcast:" #k " row_mask:0xf bank_mask:0xf\n"
-  asm("s_nop 1\n"
-      LZ_DOT4(0, 0, 5) LZ_DOT4(1, 4, 9) LZ_DOT4(2, 8, 13) LZ_DOT4(3, 12, 17)
-      LZ_DOT4(0, 1, 6) LZ_DOT4(1, 5, 10) LZ_DOT4(2, 9, 14) LZ_DOT4(3, 13, 18)
-      LZ_DOT4(0, 2, 7) LZ_DOT4(1, 6, 11) LZ_DOT4(2, 10, 15) LZ_DOT4(3, 14, 19)
-      LZ_DOT4(0, 3, 8) LZ_DOT4(1, 7, 12) LZ_DOT4(2, 11, 16) LZ_DOT4(3, 15, 20)
-      : "+&v"(y0), "+&v"(y1), "+&v"(y2), "+&v"(y3)
-      : "v"(v), "v"(h[0][0]), "v"(h[0][1]), "v"(h[0][2]), "v"(h[0][3]), "v"(h[1][0]),
-        "v"(h[1][1]), "v"(h[1][2]), "v"(h[1][3]), "v"(h[2][0]), "v"(h[2][1]), "v"(h[2][2]),
-        "v"(h[2][3]), "v"(h[3][0]), "v"(h[3][1]), "v"(h[3][2]), "v"(h[3][3]));
-#undef LZ_DOT4
-  y = f32x4{y0, y1, y2, y3};
-}
+#undef LZ_FIRST
+#undef LZ_FIRST_ADD
+#undef LZ_REST
+#undef LZ_INS
 #undef LZ_DOT
+#undef LZ_DPP
+#define LZ_DPP(op, t, k, n) \
+  op " %" #t ", %4, %" #n " row_newbcast:" #k " row_mask:0xf bank_mask:0xf\n"
+#define LZ_FIRST LZ_DPP("v_mul_f32_dpp", 0, 0, 5) LZ_DPP("v_mul_f32_dpp", 1, 4, 9) \
+  LZ_DPP("v_mul_f32_dpp", 2, 8, 13) LZ_DPP("v_mul_f32_dpp", 3, 12, 17)
+#define LZ_DOT(t, k, n) LZ_DPP("v_fmac_f32_dpp", t, k, n)
+#define LZ_FIRST_ADD LZ_DOT(0, 0, 5) LZ_DOT(1, 4, 9) LZ_DOT(2, 8, 13) LZ_DOT(3, 12, 17)
+#define LZ_REST                                                     \
+  LZ_DOT(0, 1, 6) LZ_DOT(1, 5, 10) LZ_DOT(2, 9, 14) LZ_DOT(3, 13, 18)  \
+  LZ_DOT(0, 2, 7) LZ_DOT(1, 6, 11) LZ_DOT(2, 10, 15) LZ_DOT(3, 14, 19) \
+  LZ_DOT(0, 3, 8) LZ_DOT(1, 7, 12) LZ_DOT(2, 11, 16) LZ_DOT(3, 15, 20)
+#define LZ_INS                                                                                 \
+  "v"(v), "v"(h[0][0]), "v"(h[0][1]), "v"(h[0][2]), "v"(h[0][3]), "v"(h[1][0]), "v"(h[1][1]), \
+      "v"(h[1][2]), "v"(h[1][3]), "v"(h[2][0]), "v"(h[2][1]), "v"(h[2][2]), "v"(h[2][3]),     \
+      "v"(h[3][0]), "v"(h[3][1]), "v"(h[3][2]), "v"(h[3][3])
+template <int, bool ADD>
+__device__ __forceinline__ void ssm_dots(f32x4& y, float v, const float (&h)[4][4]) {
+  float y0, y1, y2, y3;
+  if constexpr (ADD) {
+    y0 = y[0], y1 = y[1], y2 = y[2], y3 = y[3];
+    asm("s_nop 1\n" LZ_FIRST_ADD LZ_REST : "+&v"(y0), "+&v"(y1), "+&v"(y2), "+&v"(y3) : LZ_INS);
+  } else {
+    asm("s_nop 1\n" LZ_FIRST LZ_REST : "=&v"(y0), "=&v"(y1), "=&v"(y2), "=&v"(y3) : LZ_INS);
+  }
+  y = f32x4{y0, y1, y2, y3};
+}
+#undef LZ_FIRST
+#undef LZ_FIRST_ADD
+#undef LZ_REST
+#undef LZ_INS
+#undef LZ_DOT
+#undef LZ_DPP
 
 // c[n] + v(K + n) x, likewise
 template <int K>

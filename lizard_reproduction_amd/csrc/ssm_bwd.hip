@@ -292,7 +292,7 @@ __global__ __launch_bounds__(64 * (W + SSM_HELPERS), W == 8 ? 3 : 2) void ssm_bw
       const f32x4 d4 = get_tokens(sd(buf), 4 * i, lane), u4 = get_tokens(su(buf), 4 * i, lane);
       const f32x4 g4 = get_tokens(sg(buf), 4 * i, lane);
       float gs[4][2], bc16[16];
-      f32x4 dv = {0.f, 0.f, 0.f, 0.f}, du = {0.f, 0.f, 0.f, 0.f};
+      f32x4 dv = {0.f, 0.f, 0.f, 0.f}, du;
       static_for<4>([&](auto kt) {
         constexpr int t = 3 - decltype(kt)::value, tt = 4 * i + t;
         ssm_fma2<K + 2 * t>(gs[t], Cf[i >> 1], g4[t], carry);
@@ -309,7 +309,7 @@ __global__ __launch_bounds__(64 * (W + SSM_HELPERS), W == 8 ? 3 : 2) void ssm_bw
       });
       const float s = wave_sums16(bc16);
       if ((lane & 3) == i) bcsum = s;
-      ssm_dots<K>(du, Bf[i >> 1], gs);
+      ssm_dots<K, false>(du, Bf[i >> 1], gs);
       put_tokens(pd(buf, w), 4 * i, lane, dv);
       put_tokens(pu(buf, w), 4 * i, lane, du);
     });
