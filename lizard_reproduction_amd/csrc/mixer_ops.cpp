@@ -53,6 +53,13 @@ void refuse_capture(const Tensor& t) {
                              "not supported (run the kernels eagerly)");
 }
 
+// Lengths of sequences as the library takes them; 64-bit ones into [0, most] before they lose
+// their upper half
+Tensor int_lengths(const Opt& lengths, int64_t most) {
+  if (!lengths) return {};
+  return as(lengths->scalar_type() == at::kInt ? *lengths : lengths->clamp(0, most), at::kInt);
+}
+
 // Contiguous, of t's sizes and type; not given where t is not
 Tensor like(const Tensor& t) {
   return t.defined() ? at::empty(t.sizes(), t.options().memory_format(at::MemoryFormat::Contiguous))
@@ -195,7 +202,7 @@ std::tuple<Tensor, Tensor> ssm_prefill(const Tensor& x, const Tensor& dt, const 
   const c10::DeviceGuard guard(x.device());
   const SsmCall c = ssm_call(x, dt, A, B, C, get(D), get(z), get(bias), softplus);
   const Tensor in = params(get(state));
-  const Tensor lengths = lengths_ ? as(*lengths_, at::kInt) : Tensor();
+  const Tensor lengths = int_lengths(lengths_, x.size(1));
   Tensor out = at::empty({x.size(0), x.size(2), A.size(1)}, c.A.options());
   const Tensor y = c.forward(in, out, lengths, {});
   return {y.to(x.scalar_type()), out};
@@ -339,7 +346,7 @@ std::tuple<Tensor, Tensor> short_conv_prefill(const Tensor& x, const Tensor& w, 
   const c10::DeviceGuard guard(x.device());
   const ConvCall c = conv_call(x, w, get(bias), silu);
   const Tensor in = state ? as(*state, c.x.scalar_type()) : Tensor();
-  const Tensor lengths = lengths_ ? as(*lengths_, at::kInt) : Tensor();
+  const Tensor lengths = int_lengths(lengths_, x.size(1));
   const auto options = c.x.options().memory_format(at::MemoryFormat::Contiguous);
   Tensor out = at::empty({x.size(0), w.size(1) - 1, x.size(2)}, options);
   const Tensor y = c.forward(in, out, lengths);

@@ -355,6 +355,21 @@ def test_ssm_prefill_padded_batch():
     assert torch.equal(h[0].cpu(), h0[0])
 
 
+def test_lengths_past_any():
+    """Lengths below zero and past 32 bits are the sequence's ends."""
+    c, _ = _ssm_inputs(4, 20, 16, 4)
+    gpu = {k: _cuda(v) for k, v in c.items()}
+    w = torch.ones(16, 4, device="cuda")
+    for far, near in (([-1, -2 ** 31, 2 ** 31 - 1, 7], torch.int32), ([-5, -2 ** 33 + 9, 2 ** 32 + 3, 7], torch.int64)):
+        far = torch.tensor(far, dtype=near, device="cuda")
+        ends = torch.tensor([0, 0, 20, 7], dtype=torch.int32, device="cuda")
+        for a, b in zip(kernels.ssm_prefill(**gpu, lengths=far), kernels.ssm_prefill(**gpu, lengths=ends)):
+            assert torch.equal(a, b)
+        for a, b in zip(kernels.short_conv_prefill(gpu["x"], w, lengths=far),
+                        kernels.short_conv_prefill(gpu["x"], w, lengths=ends)):
+            assert torch.equal(a, b)
+
+
 def test_ssm_prefill_padded_batch_in_segments():
     """Lengths that end before, in and at segments of a split sequence."""
     c, _ = _ssm_inputs(4, 800, 24, 8)
