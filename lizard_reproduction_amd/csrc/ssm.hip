@@ -284,16 +284,19 @@ __global__ __launch_bounds__(256) void ssm_step_kernel(Ssm p, float* state) {
     if constexpr (VEC) {
       h = *reinterpret_cast<const f32x4*>(st + n0);
       a = *reinterpret_cast<const f32x4*>(A + n0);
-    }
+      Cols<T, true, 4> b4, c4;
+      b4.load(B + n0, 4), c4.load(C + n0, 4);
 #pragma unroll
-    for (int k = 0; k < 4; ++k) {
-      const int n = min(n0 + k, p.N - 1);
-      if constexpr (!VEC) {
+      for (int k = 0; k < 4; ++k) Bn[k] = b4.r.at(k), Cn[k] = c4.r.at(k);
+    } else {
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const int n = min(n0 + k, p.N - 1);
         h[k] = st[n];
         a[k] = A[n];
+        Bn[k] = (float)B[n];
+        Cn[k] = (float)C[n];
       }
-      Bn[k] = (float)B[n];
-      Cn[k] = (float)C[n];
     }
 #pragma unroll
     for (int k = 0; k < 4; ++k) {
