@@ -241,7 +241,7 @@ bool fits_step(const Tensor& x, const Tensor& state) {
 }
 
 // The step of operands that its launch takes as they are, checked here once and not in
-// Python (a step of one sequence: 17 -> 6.3 us, its kernel takes 3.4); no output for others,
+// Python (a step of one sequence: 17 -> 6.3 us, its kernel takes 3.0); no output for others,
 // which go through ssm_step after Python's checks.
 Opt ssm_step_direct(const Tensor& x, const Tensor& dt, const Tensor& A, const Tensor& B,
                     const Tensor& C, const Tensor& state, const Opt& D, const Opt& z,

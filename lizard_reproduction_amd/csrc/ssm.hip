@@ -258,67 +258,84 @@ __global__ __launch_bounds__(64 * (W + H)) void ssm_fwd_kernel(Ssm p) {
   }
 }
 
-// One token of each sequence: four lanes to a channel, lane q of them the states
-// 4 q .. 4 q + 3 of every 16, read and written once as 16 bytes.  The state's bytes bound
-// a large batch (64 sequences x 4096 channels x 16 states: 10.9 us, 36 MB at 3.3 TB/s), the
-// launch and one round of loads a small one (one sequence: 3.4 us).
-template <typename T, bool VEC>
+// One token of R sequences: four lanes to a channel, lane q of them the states 4 q .. 4 q + 3
+// of every 16, read and written once as 16 bytes.  The state's bytes bound a large batch (64
+// sequences x 4096 channels x 16 states: 9.1 us, 36 MB at 4.0 TB/s), the launch and one round
+// of loads a small one (one sequence: 2.9 us).
+template <typename T, bool VEC, int R>
 __global__ __launch_bounds__(256) void ssm_step_kernel(Ssm p, float* state) {
-  const int c = blockIdx.x * 64 + (threadIdx.x >> 2), q = threadIdx.x & 3, b = blockIdx.y;
+  const int c = blockIdx.x * 64 + (threadIdx.x >> 2), q = threadIdx.x & 3;
   const bool in = c < p.E;
   const int ci = in ? c : p.E - 1, g = ci / p.Eg;
-  const float x = (float)((const T*)p.x)[b * p.x_b + ci];
-  float d = (float)((const T*)p.dt)[b * p.dt_b + ci] + (p.bias ? p.bias[ci] : 0.f);
-  const float z = p.z ? (float)((const T*)p.z)[b * p.z_b + ci] : 0.f;
-  const float skip = p.D ? p.D[ci] * x : 0.f;
-  const T* B = (const T*)p.B + b * p.B_b + (long long)g * p.B_g;
-  const T* C = (const T*)p.C + b * p.C_b + (long long)g * p.C_g;
+  const float bias = p.bias ? p.bias[ci] : 0.f, D = p.D ? p.D[ci] : 0.f;
   const float* A = p.A + (size_t)ci * p.N;
-  float* st = state + ((size_t)b * p.E + ci) * p.N;
-  if (p.softplus) d = softplus(d);
-  const float u = d * x;
-  float y = 0.f;
+  float x[R], d[R], z[R], y[R];
+  int b[R];
+#pragma unroll
+  for (int r = 0; r < R; ++r) {
+    b[r] = min((int)blockIdx.y * R + r, p.batch - 1);   // past the last one, it again
+    x[r] = (float)((const T*)p.x)[b[r] * p.x_b + ci];
+    d[r] = (float)((const T*)p.dt)[b[r] * p.dt_b + ci];
+    z[r] = p.z ? (float)((const T*)p.z)[b[r] * p.z_b + ci] : 0.f;
+    y[r] = 0.f;
+  }
   for (int n0 = 4 * q; n0 < p.N; n0 += 16) {
-    f32x4 h, a;
-    float Bn[4], Cn[4];
-    if constexpr (VEC) {
-      h = *reinterpret_cast<const f32x4*>(st + n0);
-      a = *reinterpret_cast<const f32x4*>(A + n0);
-      Cols<T, true, 4> b4, c4;
-      b4.load(B + n0, 4), c4.load(C + n0, 4);
+    f32x4 h[R], a;
+    float Bn[R][4], Cn[R][4];
+    if constexpr (VEC) a = *reinterpret_cast<const f32x4*>(A + n0);
 #pragma unroll
-      for (int k = 0; k < 4; ++k) Bn[k] = b4.r.at(k), Cn[k] = c4.r.at(k);
-    } else {
+    for (int r = 0; r < R; ++r) {
+      const float* st = state + ((size_t)b[r] * p.E + ci) * p.N;
+      const T* B = (const T*)p.B + b[r] * p.B_b + (long long)g * p.B_g;
+      const T* C = (const T*)p.C + b[r] * p.C_b + (long long)g * p.C_g;
+      if constexpr (VEC) {
+        h[r] = *reinterpret_cast<const f32x4*>(st + n0);
+        Cols<T, true, 4> b4, c4;
+        b4.load(B + n0, 4), c4.load(C + n0, 4);
 #pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        const int n = min(n0 + k, p.N - 1);
-        h[k] = st[n];
-        a[k] = A[n];
-        Bn[k] = (float)B[n];
-        Cn[k] = (float)C[n];
+        for (int k = 0; k < 4; ++k) Bn[r][k] = b4.r.at(k), Cn[r][k] = c4.r.at(k);
+      } else {
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          const int n = min(n0 + k, p.N - 1);
+          h[r][k] = st[n];
+          a[k] = A[n];
+          Bn[r][k] = (float)B[n];
+          Cn[r][k] = (float)C[n];
+        }
       }
     }
 #pragma unroll
-    for (int k = 0; k < 4; ++k) {
-      h[k] = fmaf(__builtin_amdgcn_exp2f(d * (a[k] * LOG2E)), h[k], u * Bn[k]);
-      if (n0 + k < p.N) y = fmaf(Cn[k], h[k], y);
-    }
-    if (in) {
-      if constexpr (VEC) {
-        *reinterpret_cast<f32x4*>(st + n0) = h;
-      } else {
+    for (int r = 0; r < R; ++r) {
+      float delta = d[r] + bias;
+      if (p.softplus) delta = softplus(delta);
+      const float u = delta * x[r];
 #pragma unroll
-        for (int k = 0; k < 4; ++k)
-          if (n0 + k < p.N) st[n0 + k] = h[k];
+      for (int k = 0; k < 4; ++k) {
+        h[r][k] = fmaf(__builtin_amdgcn_exp2f(delta * (a[k] * LOG2E)), h[r][k], u * Bn[r][k]);
+        if (n0 + k < p.N) y[r] = fmaf(Cn[r][k], h[r][k], y[r]);
+      }
+      float* st = state + ((size_t)b[r] * p.E + ci) * p.N;
+      if (in && (R == 1 || (int)blockIdx.y * R + r < p.batch)) {
+        if constexpr (VEC) {
+          *reinterpret_cast<f32x4*>(st + n0) = h[r];
+        } else {
+#pragma unroll
+          for (int k = 0; k < 4; ++k)
+            if (n0 + k < p.N) st[n0 + k] = h[r][k];
+        }
       }
     }
   }
-  y += dpp<DPP_XOR1>(y);
-  y += dpp<DPP_XOR2>(y);
-  if (q == 0 && in) {
-    y += skip;
-    if (p.z) y *= z * sigmoid(z);
-    ((T*)p.y)[(size_t)b * p.E + c] = (T)y;
+#pragma unroll
+  for (int r = 0; r < R; ++r) {
+    y[r] += dpp<DPP_XOR1>(y[r]);
+    y[r] += dpp<DPP_XOR2>(y[r]);
+    if (q == 0 && in) {
+      float o = fmaf(D, x[r], y[r]);
+      if (p.z) o *= z[r] * sigmoid(z[r]);
+      ((T*)p.y)[(size_t)b[r] * p.E + c] = (T)o;
+    }
   }
 }
 
@@ -373,18 +390,23 @@ hipError_t launch_ssm_fwd(const Ssm& p, bool is_bf16, bool vec, hipStream_t st) 
   return vec ? fwd_waves<float, true>(p, st) : fwd_waves<float, false>(p, st);
 }
 
-hipError_t launch_ssm_step(const Ssm& p, float* state, bool is_bf16, hipStream_t st) {
-  const dim3 grid((p.E + 63) / 64, p.batch);
-  const bool vec = p.N % 4 == 0 && ((uintptr_t)state | (uintptr_t)p.A) % 16 == 0;
-  if (is_bf16 && vec)
-    hipLaunchKernelGGL((ssm_step_kernel<bf16, true>), grid, dim3(256), 0, st, p, state);
-  else if (is_bf16)
-    hipLaunchKernelGGL((ssm_step_kernel<bf16, false>), grid, dim3(256), 0, st, p, state);
-  else if (vec)
-    hipLaunchKernelGGL((ssm_step_kernel<float, true>), grid, dim3(256), 0, st, p, state);
+template <typename T, int R>
+hipError_t step_launch(const Ssm& p, float* state, hipStream_t st) {
+  const dim3 grid((p.E + 63) / 64, (p.batch + R - 1) / R);
+  if (p.N % 4 == 0 && ((uintptr_t)state | (uintptr_t)p.A) % 16 == 0)
+    hipLaunchKernelGGL((ssm_step_kernel<T, true, R>), grid, dim3(256), 0, st, p, state);
   else
-    hipLaunchKernelGGL((ssm_step_kernel<float, false>), grid, dim3(256), 0, st, p, state);
+    hipLaunchKernelGGL((ssm_step_kernel<T, false, R>), grid, dim3(256), 0, st, p, state);
   return hipGetLastError();
+}
+
+// Two sequences a thread from as many workgroups on as the chip holds at once, eight a CU
+// (4096 channels x 16 states: 64 sequences 9.1 us, with one a thread 10.4; 32: 5.9 and 6.2;
+// 16: 4.6 and 4.3; one: 3.2 and 2.9)
+hipError_t launch_ssm_step(const Ssm& p, float* state, bool is_bf16, hipStream_t st) {
+  if ((p.E + 63LL) / 64 * p.batch >= 8LL * device_geom().cus)
+    return is_bf16 ? step_launch<bf16, 2>(p, state, st) : step_launch<float, 2>(p, state, st);
+  return is_bf16 ? step_launch<bf16, 1>(p, state, st) : step_launch<float, 1>(p, state, st);
 }
 
 }  // namespace lz

@@ -249,6 +249,28 @@ def test_steps_of_operands_in_any_form():
     check(h, *want["state"], 264, "step mixed state")
 
 
+@pytest.mark.parametrize("n, dtype", [(16, BF16), (24, FP32), (5, BF16)])
+def test_steps_of_many_sequences(n, dtype):
+    """Batches that fill the GPU, odd ones among them: each sequence's step is, to the bit, the
+    step of it alone, and the memory after the last sequence stays as it was."""
+    e = 1000
+    for b in (127, 128, 129, 257):
+        g = torch.Generator("cuda").manual_seed(b)
+        x, dt, z = (torch.randn(b, e, device="cuda", dtype=dtype, generator=g) for _ in range(3))
+        B, C = (torch.randn(b, n, device="cuda", dtype=dtype, generator=g) for _ in range(2))
+        A = -torch.rand(e, n, device="cuda", generator=g)
+        D = torch.randn(e, device="cuda", generator=g)
+        states = torch.randn(b + 2, e, n, device="cuda", generator=g)
+        kept = states.clone()
+        y = kernels.ssm_decode_step(x, dt, A, B, C, states[:b], D=D, z=z)
+        assert torch.equal(states[b:], kept[b:])
+        for i in (0, 1, b // 2, b - 2, b - 1):
+            h = kept[i:i + 1].clone()
+            row = kernels.ssm_decode_step(x[i:i + 1], dt[i:i + 1], A, B[i:i + 1], C[i:i + 1], h, D=D,
+                                          z=z[i:i + 1])
+            assert torch.equal(row[0], y[i]) and torch.equal(h[0], states[i]), (b, i)
+
+
 def test_steps_write_their_state_alone():
     """States as slots of a larger cache: the slots beside them stay as they were."""
     cache = torch.randn(5, 64, 16, device="cuda")
