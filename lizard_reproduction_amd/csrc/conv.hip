@@ -7,8 +7,8 @@
 // K rows in registers: a row is read once by the run it lies in, and its last K - 1 again,
 // from cache, by the run after it.  A workgroup's threads are columns of vectors times runs,
 // a row's columns next to each other.  bf16, K = 4, 8192 tokens x 4096 channels: the forward
-// takes 28.7 us, 134 MB at 4.7 TB/s, the backward 45 us, 201 MB at 4.5 TB/s, where a copy
-// runs at 4.9; the last launch, which adds the runs' shares of dw and dbias, 4 us.
+// takes 28.7 us, 134 MB at 4.7 TB/s, the backward 42.7 us, 201 MB at 4.7 TB/s, where a copy
+// runs at 4.9; the last launch, which adds the runs' shares of dw and dbias, 4.6 us.
 //
 // Backward: g_t = dy_t act'(pre_t), dx_t = sum_j w_j g_{t+K-1-j} (the run goes K - 1 tokens
 // on), dw_j = sum_t g_t x_{t-K+1+j}, dbias = sum_t g_t: the workgroup's runs meet in LDS and
@@ -261,9 +261,9 @@ __global__ __launch_bounds__(CONV_THREADS) void conv_bwd_kernel(Conv p, const vo
 }
 
 // Runs long enough that their K - 1 rows before them cost little, short enough that the
-// threads fill the chip twice over.  (Threads a CU, training 8192 tokens x 4096 channels and
-// a forward of 5 x 1021 x 2050: 256 took 82 and 27 us, 512 81 and 15, 1024 85 and 15; runs of
-// at most 32, 64 and 128 tokens 82, 81 and 83 us of the first.)
+// threads fill the chip: two workgroups a CU in the forward (8192 tokens x 4096 channels: 28.9
+// us, with 1.5, 3 and 4 a CU 32.7, 31.0 and 33.1), four in the backward (42.7 us, with 2, 3
+// and 8 45.4, 43.9 and 47.3).  Runs of at most 32, 64 and 128 tokens made 1 % of a difference.
 void conv_split(Conv& p, bool backward) {
   const int V = backward ? CONV_BWD_V : CONV_FWD_V, vecs = (p.C + V - 1) / V;
   int cols = 1;
@@ -274,7 +274,7 @@ void conv_split(Conv& p, bool backward) {
   p.cols = cols;
   p.col_blocks = (vecs + cols - 1) / cols;
   const long long rows = (long long)p.batch * p.L;
-  const long long threads = 512LL * device_geom().cus;
+  const long long threads = (backward ? 1024LL : 512LL) * device_geom().cus;
   long long run = rows * vecs / threads;
   run = run < 8 ? 8 : run > 64 ? 64 : run;
   run = (run + CONV_AHEAD - 1) / CONV_AHEAD * CONV_AHEAD;
